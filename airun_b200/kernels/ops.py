@@ -57,6 +57,13 @@ def _cuda(*ts: Optional[torch.Tensor]) -> None:
             _need(t.is_cuda, "kernel arguments must live on the GPU (there is no CPU path)")
 
 
+def _one_device(*ts: Optional[torch.Tensor]) -> None:
+    """All on the current device, whose stream the kernel is launched on."""
+    here = torch.cuda.current_device()
+    for t in ts:
+        _need(t is None or t.device.index == here, "kernel arguments must live on the current device")
+
+
 LAUNCHES = [0]          # kernels launched through this module (CUDA-graph replays are counted by their owner)
 
 
@@ -91,7 +98,7 @@ def required_libraries(dtype: torch.dtype, head_dim: int):
     libs = [("elementwise", None), ("gemm_simt", None), ("qkv_post", None),
             ("attention_generic", None), ("sampling", None), ("linear_attention", None), ("diff_attention", None),
             ("recurrent_state", None), ("latent_attention", None), ("moe", None), ("sigmoid_attention", None),
-            ("streams", None), ("softmax_attention", None)]
+            ("streams", None), ("softmax_attention", None), ("logprobs", None)]
     return libs
 
 
@@ -1258,6 +1265,58 @@ def largest_logits(logits: torch.Tensor, rows: torch.Tensor, n: int, n_cand: int
             [c_void_p, c_longlong, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p])
     _check(f(_p(logits), logits.stride(0) if R > 1 else max(V, logits.stride(0)), V, _p(rows), int(n), int(n_cand),
              _p(out_ids), _p(out_vals), _p(out_flags), _stream()), "largest_logits")
+
+
+TOP_LOGPROBS_MAX = 128
+
+
+def _logprob_outputs(tokens: torch.Tensor, vocab: int, logprob, entropy, lse, top_ids, top_logprobs) -> int:
+    """Checks the given tokens and the places for their results; returns how many alternatives are asked for."""
+    _cuda(tokens, logprob, entropy, lse, top_ids, top_logprobs)
+    _need(tokens.dtype == torch.int32 and tokens.dim() == 1 and tokens.is_contiguous(), "tokens must be int32 [n]")
+    n = tokens.shape[0]
+    for t in (logprob, entropy, lse):
+        _need(t is None or (t.dtype == torch.float32 and tuple(t.shape) == (n,) and t.is_contiguous()),
+              "logprob, entropy and lse must be float32 [n]")
+    _need((top_ids is None) == (top_logprobs is None), "the alternatives' ids and log probabilities come together")
+    if top_ids is None:
+        return 0
+    _need(top_ids.dim() == 2 and top_ids.shape[0] == n and 1 <= top_ids.shape[1] <= min(TOP_LOGPROBS_MAX, vocab),
+          f"the alternatives are [n, k] with k from 1 to {TOP_LOGPROBS_MAX} and to the vocabulary")
+    _need(top_ids.dtype == torch.int32 and top_ids.is_contiguous() and top_logprobs.dtype == torch.float32
+          and top_logprobs.shape == top_ids.shape and top_logprobs.is_contiguous(),
+          "the alternatives' ids must be int32 and their log probabilities float32, contiguous and of one shape")
+    return top_ids.shape[1]
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tensor, entropy: Optional[torch.Tensor] = None,
+                   lse: Optional[torch.Tensor] = None, top_ids: Optional[torch.Tensor] = None,
+                   top_logprobs: Optional[torch.Tensor] = None, rows: Optional[torch.Tensor] = None,
+                   err: Optional[torch.Tensor] = None) -> None:
+    """Log probabilities of given tokens under softmax(logits), with the row's entropy (nats), ln sum exp (``lse``) and its
+    likeliest tokens, each where a place for it is given.
+
+    logits: [R, V] float32 or bfloat16, rows any distance apart; tokens: int32 [n] on the device, one a row; ``rows``: int32 [n],
+    the rows that are meant (None: row i for token i, R >= n); logprob, entropy, lse: float32 [n]; top_ids int32 and top_logprobs
+    float32 [n, k]: the k largest logits, the largest first and equal ones by ascending id.
+
+    NaN counts as minus infinity.  A row with nothing above minus infinity has log probabilities of minus infinity and the
+    entropy 0, one with plus infinity the entropy NaN; a token outside [0, V) has minus infinity, so rows that are padding may ask for
+    -1.  A row index outside [0, R) reads nothing: it gives what a row without a distribution does, with ids of -1, and sets
+    the bit of a bad row in ``err``, if that is given."""
+    _cuda(logits, rows, err)
+    _need(logits.dim() == 2 and logits.shape[1] > 0 and logits.stride(1) == 1, "logits must be row-major [rows, V]")
+    R, V = logits.shape
+    k = _logprob_outputs(tokens, V, logprob, entropy, lse, top_ids, top_logprobs)
+    n = tokens.shape[0]
+    _need(rows is None or (rows.dtype == torch.int32 and tuple(rows.shape) == (n,) and rows.is_contiguous()), "rows must be int32 [n]")
+    _need(rows is not None or R >= n, "a row of logits for every token")
+    _need(R <= 1 or logits.stride(0) >= V, "rows of logits must not overlap")
+    _one_device(logits, tokens, logprob, entropy, lse, top_ids, top_logprobs, rows, err)
+    f = _fn("logprobs", "airun_token_logprobs", [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                                                 c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p])
+    _check(f(_p(logits), _dt(logits), logits.stride(0) if R > 1 else V, R, V, _p(rows), _p(tokens), n, _p(logprob), _p(entropy), _p(lse), k,
+             _p(top_ids), _p(top_logprobs), _p(err), _stream()), "token_logprobs")
 
 
 def describe_device_error(bits: int) -> str:

@@ -1,0 +1,239 @@
+"""Log probabilities of given tokens, entropies and alternatives against plain formulas in 64 bits.
+
+Tolerances.  A result is built from m (a logit, exact), s and u.  The terms exp(x - m) are off by a few units of 2^-24 times
+(1 + |x - m|), for |x - m| up to 20 (what is further down adds less than 2e-9) at most 4e-6 each with any sign, and a sum of V terms kept in V / 512 steps
+and joined over threads by up to V / 512 * 2^-24 relative (2e-5 at 160,000 would be the bound if all had one sign; rounding to nearest leaves its
+root, 1e-6).  So ln s and u / s are off by about 5e-6 times 1 + their size, and 2e-5 * (1 + |result|) holds every case with a margin;
+ids have no tolerance at all."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+DEV = "cuda"
+
+
+def plain(x, tokens, k):
+    """x: float64 [n, V] on the CPU."""
+    n, V = x.shape
+    x = torch.where(torch.isnan(x), torch.full_like(x, -math.inf), x)
+    m = x.amax(1, keepdim=True)
+    some = (m > -math.inf)[:, 0]
+    d = torch.where(x > -math.inf, x - torch.where(m > -math.inf, m, torch.zeros_like(m)), torch.full_like(x, -math.inf))
+    e = torch.exp(d)
+    s = e.sum(1)
+    ln_s = torch.log(s)
+    lse = torch.where(some, m[:, 0] + ln_s, torch.full_like(ln_s, -math.inf))
+    H = torch.where(some, ln_s - torch.where(e > 0, e * d, torch.zeros_like(e)).sum(1) / s, torch.zeros_like(s))
+    lp = torch.where(some[:, None], d - torch.where(some, ln_s, torch.zeros_like(s))[:, None], torch.full_like(x, -math.inf))
+    t = tokens.long()
+    got = torch.where((t >= 0) & (t < V), lp.gather(1, t.clamp(0, V - 1)[:, None])[:, 0], torch.full((n,), -math.inf, dtype=torch.float64))
+    order = torch.from_numpy(np.argsort(-x.numpy(), axis=1, kind="stable")[:, :k].copy())      # equal logits by ascending id
+    return got, H, lse, order, lp.gather(1, order)
+
+
+def call(logits, tokens, k, rows=None, err=None):
+    from airun_b200.kernels import ops
+    n = tokens.shape[0]
+    lp, H, lse = (torch.full((n,), 7.0, device=DEV) for _ in range(3))
+    ids = torch.full((n, k), -7, dtype=torch.int32, device=DEV) if k else None
+    tops = torch.full((n, k), 7.0, device=DEV) if k else None
+    ops.token_logprobs(logits, tokens, lp, H, lse, ids, tops, rows=rows, err=err)
+    torch.cuda.synchronize()
+    return [None if t is None else t.cpu() for t in (lp, H, lse, ids, tops)]
+
+
+def near(got, want, tol=2e-5):
+    got = got.double()
+    fine = torch.isfinite(want)
+    assert torch.equal(fine, torch.isfinite(got)) and torch.equal(got[~fine], want[~fine]), (got[~fine], want[~fine])
+    off = (got[fine] - want[fine]).abs() / (1 + want[fine].abs())
+    assert off.numel() == 0 or float(off.max()) <= tol, float(off.max())
+
+
+def check(logits, tokens, k, rows=None, tol=2e-5):
+    got = call(logits, tokens, k, rows)
+    x = (logits if rows is None else logits[rows.long()]).double().cpu()[: tokens.shape[0]]
+    want = plain(x, tokens.cpu(), k)
+    for g, w in zip(got[:3], want[:3]):
+        near(g, w, tol)
+    if k:
+        assert torch.equal(got[3].long(), want[3])
+        near(got[4], want[4], tol)
+    return got
+
+
+def some_tokens(n, V, seed):
+    t = torch.randint(0, V, (n,), generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+    if n > 2:
+        t[1], t[2] = -1, V                            # a padded row, an id behind the vocabulary
+    return t.to(DEV)
+
+
+SIZES = [(1, 1, 1), (3, 2, 2), (5, 31, 31), (4, 129, 128), (7, 384, 5), (2, 2047, 9), (2, 2048, 40), (2, 2049, 8), (3, 4099, 3), (1, 8192, 1), (1, 16411, 20),
+         (9, 50001, 33), (1, 151936, 5), (40, 65537, 128), (300, 5000, 20), (700, 1000, 0), (149, 33000, 2)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,V,k", SIZES)
+def test_tokens_against_64_bits(n, V, k, dtype):
+    g = torch.Generator().manual_seed(n * 7919 + V)
+    x = (torch.randn(n, V, generator=g) * 3).to(dtype).to(DEV)     # bfloat16: many equal logits
+    check(x, some_tokens(n, V, V), k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("pad,lead", [(1, 0), (3, 1), (5, 3), (8, 7)])
+def test_tokens_any_stride_and_alignment(dtype, pad, lead):
+    g = torch.Generator().manual_seed(pad)
+    buf = torch.full((6, 9000 + pad + lead), 99.0)                 # what lies between the rows must not be read as a logit
+    buf[:, lead:lead + 9000] = torch.randn(6, 9000, generator=g)
+    x = buf.to(dtype).to(DEV)[:, lead:lead + 9000]
+    check(x, some_tokens(6, 9000, pad), 11)
+    check(x[:1], some_tokens(1, 9000, pad), 11)
+    check(x[:, :700], some_tokens(6, 700, pad), 11)
+
+
+@pytest.mark.gpu
+def test_tokens_of_picked_rows_and_bad_rows():
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(12, 6000, generator=g).to(DEV)
+    rows = torch.tensor([11, 0, 7, 7, 3], dtype=torch.int32, device=DEV)                 # one row twice, for two tokens
+    check(x, some_tokens(5, 6000, 4), 4, rows=rows)
+    from airun_b200.kernels import ops
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    rows = torch.tensor([2, -1, 12], dtype=torch.int32, device=DEV)
+    lp, H, lse, ids, tops = call(x, some_tokens(3, 6000, 4).clamp(0, 5999), 4, rows, err)
+    assert math.isfinite(lp[0]) and lp[1:].tolist() == [-math.inf] * 2 and H[1:].tolist() == [0.0, 0.0] and lse[1:].tolist() == [-math.inf] * 2
+    assert ids[1:].tolist() == [[-1] * 4] * 2 and tops[1:].tolist() == [[-math.inf] * 4] * 2
+    assert int(err.item()) == 16 and "row" in ops.describe_device_error(16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [300, 7001, 70001])
+def test_tokens_masks_ties_and_not_a_number(dtype, V):
+    low = torch.finfo(dtype).min
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(14, V, generator=g)
+    x[0] = -math.inf                                   # nothing is left
+    x[1] = math.nan
+    x[2] = 0.0                                         # all equal
+    x[3] = low                                         # all at the type's lowest value: still a distribution
+    x[4, 5:] = -math.inf                               # fewer than k
+    x[5, : V - 3] = low
+    x[6, ::2] = math.nan
+    x[7, 17] = math.inf
+    x[8] = -0.0
+    x[8, ::3] = 0.0                                    # zeros of both signs are equal
+    x[9] = torch.arange(V) * (60.0 / V)                # sorted
+    x[10] = -torch.arange(V) * (60.0 / V)
+    x[11] *= 1000.0                                    # far apart
+    x[12, V // 2:] = torch.finfo(dtype).max
+    x[13] = (torch.arange(V) % 512 == 3).float() * 5   # the largest ones repeat at the threads' stride
+    x = x.to(dtype).to(DEV)
+    t = torch.full((14,), 4, dtype=torch.int32, device=DEV)
+    keep = [i for i in range(14) if i != 7]
+    for k in (0, 1, 7, 32, 100):
+        check(x[keep].contiguous(), t[keep], k)
+        lp, H, lse, ids, tops = call(x[7:8].contiguous(), t[7:8], k)
+        assert lp[0] == -math.inf and math.isnan(H[0]) and lse[0] == math.inf
+        if k:
+            assert ids[0, 0] == 17 and math.isnan(tops[0, 0]) and bool((tops[0, 1:] == -math.inf).all())
+    one = torch.full((1, V), -math.inf)
+    one[0, V - 2] = 3.0
+    got = check(one.to(dtype).to(DEV), torch.tensor([V - 2], dtype=torch.int32, device=DEV), 3)
+    assert got[0][0] == 0.0 and got[1][0] == 0.0 and got[3][0].tolist() == [V - 2, 0, 1]
+
+
+@pytest.mark.gpu
+def test_tokens_rows_far_into_a_large_buffer():
+    """Row 17,000 of 131,072 columns lies behind 2^31 elements."""
+    V = 131072
+    x = torch.empty(17001, V, dtype=torch.bfloat16, device=DEV)
+    x[17000] = torch.randn(V, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+    rows = torch.tensor([17000], dtype=torch.int32, device=DEV)
+    got = call(x, torch.tensor([77], dtype=torch.int32, device=DEV), 6, rows)
+    want = plain(x[17000:].double().cpu(), torch.tensor([77]), 6)
+    near(got[0], want[0])
+    assert torch.equal(got[3].long(), want[3])
+
+
+@pytest.mark.gpu
+def test_tokens_leave_rows_behind_the_last_alone_and_repeat_bit_for_bit():
+    from airun_b200.kernels import ops
+    x = torch.randn(30, 20000, generator=torch.Generator().manual_seed(5)).to(DEV)
+    t = some_tokens(30, 20000, 1)
+    lp, ids, tops = torch.full((40,), 7.0, device=DEV), torch.full((40, 3), -7, dtype=torch.int32, device=DEV), torch.full((40, 3), 7.0, device=DEV)
+    kept = []
+    for _ in range(3):
+        ops.token_logprobs(x, t, lp[:30], top_ids=ids[:30], top_logprobs=tops[:30])
+        kept.append((lp.clone(), ids.clone(), tops.clone()))
+    assert lp[30:].unique().tolist() == [7.0] and ids[30:].unique().tolist() == [-7] and tops[30:].unique().tolist() == [7.0]
+    for got in kept[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got, kept[0]))
+    ops.token_logprobs(x[:0], t[:0], lp[:0])            # no rows: nothing happens
+
+
+@pytest.mark.gpu
+def test_tokens_on_another_stream_and_in_two_graphs():
+    from airun_b200.kernels import ops
+    x = torch.randn(6, 40000, generator=torch.Generator().manual_seed(8)).to(DEV)
+    t = some_tokens(6, 40000, 2)
+    want = call(x, t, 5)
+    places = [(torch.empty(6, device=DEV), torch.empty(6, 5, dtype=torch.int32, device=DEV), torch.empty(6, 5, device=DEV)) for _ in range(2)]
+    graphs = []
+    torch.cuda.synchronize()
+    for lp, ids, tops in places:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ops.token_logprobs(x, t, lp, top_ids=ids, top_logprobs=tops)
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for lp, ids, tops in places:
+        assert torch.equal(lp.cpu(), want[0]) and torch.equal(ids.cpu(), want[3]) and torch.equal(tops.cpu(), want[4])
+
+
+class _Fake:
+    """A tensor's stand-in that says it is on the GPU, for the checks that come before any launch."""
+
+    def __new__(cls, *shape, dtype=torch.float32):
+        t = torch.empty(*shape, dtype=dtype)
+
+        class OnGpu(torch.Tensor):
+            is_cuda = True
+        return t.as_subclass(OnGpu)
+
+
+def test_refusals(monkeypatch):
+    from airun_b200.kernels import ops
+    monkeypatch.setattr(ops, "_fn", lambda *a, **k: pytest.fail("launched"))
+    monkeypatch.setattr(ops, "_one_device", lambda *a: None)
+    x, t, lp = _Fake(4, 100), _Fake(4, dtype=torch.int32), _Fake(4)
+
+    def refused(match, logits=x, tokens=t, logprob=lp, **kw):
+        with pytest.raises(ops.KernelError, match=match):
+            ops.token_logprobs(logits, tokens, logprob, **kw)
+
+    refused("GPU", logits=torch.empty(4, 100))
+    refused("int32", tokens=_Fake(4, dtype=torch.int64))
+    refused("float32", logprob=_Fake(3))
+    refused("float32", entropy=_Fake(4, dtype=torch.float64))
+    refused("every token", logits=_Fake(3, 100))
+    refused("row-major", logits=_Fake(100, 4).t())
+    refused("overlap", logits=_Fake(400).as_strided((4, 100), (50, 1)))
+    refused("together", top_ids=_Fake(4, 3, dtype=torch.int32))
+    refused("to the vocabulary", top_ids=_Fake(4, 101, dtype=torch.int32), top_logprobs=_Fake(4, 101))
+    refused("to the vocabulary", logits=_Fake(4, 999), top_ids=_Fake(4, 129, dtype=torch.int32), top_logprobs=_Fake(4, 129))
+    refused("one shape", top_ids=_Fake(4, 3, dtype=torch.int32), top_logprobs=_Fake(4, 2))
+    refused("int32", rows=_Fake(5, dtype=torch.int32))
+    monkeypatch.setattr(ops, "_fn", lambda *a, **k: (lambda *b: 0))
+    refused("dtype", logits=_Fake(4, 100, dtype=torch.float16))
