@@ -369,6 +369,18 @@ def linear_bf16(ctx, x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, normed
     return True
 
 
+def linear_unsliced_bf16(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, err: torch.Tensor) -> bool:
+    """out = x @ w^T, float32, without slices that meet in scratch: for callers that may run beside others."""
+    if not _usable(x, w):
+        return False
+    M, N = x.shape[0], w.shape[0]
+    if M > 64 and "gemm_pair" not in DISABLED:
+        gemm_pair(x, w, out, EPI_F32, err, in_parts=x.shape[1] > 512)
+    else:
+        gemm_tcgen05(x, w, out, EPI_F32, True, 16 if M <= 16 else 32 if M <= 32 else 64 if M <= 64 else 128, 1, err)
+    return True
+
+
 def linear_swiglu_bf16(ctx, x: torch.Tensor, w_gu: torch.Tensor, out: torch.Tensor, group: int, normed=None) -> bool:
     if group != 16 or not _usable(x, w_gu) or w_gu.shape[0] % 32 != 0:
         return False

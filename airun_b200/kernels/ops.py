@@ -1319,5 +1319,57 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Te
              _p(top_ids), _p(top_logprobs), _p(err), _stream()), "token_logprobs")
 
 
+_cap = soft_cap                        # (an argument has the name below)
+HEAD_CHUNK = 1 << 26                   # logits that are held at a time where they are formed at all: 256 MiB
+
+
+def head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tensor, err: torch.Tensor,
+                  entropy: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, top_ids: Optional[torch.Tensor] = None,
+                  top_logprobs: Optional[torch.Tensor] = None, scale: float = 1.0, soft_cap: Optional[float] = None, ws=None) -> None:
+    """``token_logprobs`` of the logits hidden @ weight^T, times ``scale`` and capped to soft_cap * tanh(logits / soft_cap), without a
+    place for them: hidden [n, H] and weight [V, H], both float32 or both bfloat16, row-major; the other arguments as there.
+
+    ``ws``: an engine.batch.Workspace to take scratch from (None: allocated).  Scratch is in use until the call's kernels are done:
+    calls that may overlap on the GPU (two streams, two graphs) need workspaces of their own.  ``err``: int32 [1], the device-side
+    error word."""
+    _cuda(hidden, weight, err)
+    _need(hidden.dim() == 2 and weight.dim() == 2 and hidden.shape[1] == weight.shape[1] and weight.shape[0] > 0 and weight.shape[1] > 0,
+          "hidden [n, H] and weight [V, H] do not agree")
+    _need(hidden.dtype == weight.dtype, "hidden and weight must share a type")
+    _need(hidden.stride(1) == 1 and weight.stride(1) == 1, "hidden and weight must be row-major")
+    n, V = hidden.shape[0], weight.shape[0]
+    _need(tokens.dim() == 1 and tokens.shape[0] == n, "a token for every row")
+    k = _logprob_outputs(tokens, V, logprob, entropy, lse, top_ids, top_logprobs)
+    _need(err.dtype == torch.int32 and err.numel() == 1, "err must be one int32")
+    _need(scale == scale and abs(scale) < float("inf"), "the scale must be finite")
+    _need(soft_cap is None or 0.0 < soft_cap < float("inf"), "the cap must be positive")
+    _dt(hidden)
+    _one_device(hidden, weight, tokens, logprob, entropy, lse, top_ids, top_logprobs, err)
+    if n == 0:
+        return
+    alloc = ws.alloc if ws is not None else (lambda shape, dtype: torch.empty(shape, dtype=dtype, device=hidden.device))
+    step = min(n, max(1, HEAD_CHUNK // V))
+    logits = alloc((step, V), torch.float32)
+    for a in range(0, n, step):
+        b = min(n, a + step)
+        x = logits[:b - a]
+        _head_product(hidden[a:b], weight, x, err)
+        if scale != 1.0:
+            scale_(x, scale)
+        if soft_cap is not None:
+            _cap(x, soft_cap)
+        part = lambda t: None if t is None else t[a:b]      # noqa: E731
+        token_logprobs(x, tokens[a:b], logprob[a:b], part(entropy), part(lse), part(top_ids), part(top_logprobs))
+
+
+def _head_product(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, err: torch.Tensor) -> None:
+    """out = x @ w^T in float32 by a kernel that needs no scratch (that of the products in slices belongs to one stream)."""
+    if x.dtype == torch.bfloat16:
+        from . import fast
+        if fast.linear_unsliced_bf16(x, w, out, err):
+            return
+    gemm_simt(x, w, out, err)
+
+
 def describe_device_error(bits: int) -> str:
     return "; ".join(msg for b, msg in DEV_ERR_BITS.items() if bits & b) or f"unknown error bits {bits}"

@@ -202,6 +202,152 @@ def test_tokens_on_another_stream_and_in_two_graphs():
         assert torch.equal(lp.cpu(), want[0]) and torch.equal(ids.cpu(), want[3]) and torch.equal(tops.cpu(), want[4])
 
 
+# ---------------------------------------------------------------- from hidden states
+def head(h, w, tokens, k, scale=1.0, cap=None, ws=None, **kw):
+    from airun_b200.kernels import ops
+    n = h.shape[0]
+    lp, H, lse = (torch.full((n,), 7.0, device=DEV) for _ in range(3))
+    ids = torch.full((n, k), -7, dtype=torch.int32, device=DEV) if k else None
+    tops = torch.full((n, k), 7.0, device=DEV) if k else None
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ops.head_logprobs(h, w, tokens, lp, err, H, lse, ids, tops, scale=scale, soft_cap=cap, ws=ws)
+    torch.cuda.synchronize()
+    assert int(err.item()) == 0
+    return [None if t is None else t.cpu() for t in (lp, H, lse, ids, tops)]
+
+
+def grid_inputs(n, H, V, dtype, seed):
+    """Multiples of 1/4 up to 1 and of 1/64 up to 1/8: every sum of up to 8,192 products is a multiple of 1/256 below 1,024 and
+    exact in 32 bits in any order, so the logits have no rounding and many of them are equal."""
+    g = torch.Generator().manual_seed(seed)
+    h = torch.randint(-4, 5, (n, H), generator=g).float() / 4
+    w = torch.randint(-8, 9, (V, H), generator=g).float() / 64
+    return h.to(dtype).to(DEV), w.to(dtype).to(DEV)
+
+
+HEAD_SIZES = [(1, 64, 1, 1), (1, 8, 300, 3), (2, 4096, 5000, 5), (5, 72, 257, 16), (8, 1024, 20000, 0), (64, 200, 4000, 4), (100, 512, 16400, 1), (127, 64, 384, 3),
+              (128, 1032, 33, 16), (129, 520, 1000, 2), (256, 96, 2049, 5), (257, 2048, 1500, 8), (700, 1024, 20000, 0), (1111, 64, 700, 2), (3, 64, 160000, 7),
+              (300, 136, 40000, 16), (5, 256, 5000, 40), (200, 72, 3001, 100)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,H,V,k", HEAD_SIZES)
+def test_head_exact_logits(n, H, V, k, dtype):
+    h, w = grid_inputs(n, H, V, dtype, n + H + V)
+    t = some_tokens(n, V, n)
+    got = head(h, w, t, k)
+    want = plain(h.double().cpu() @ w.double().cpu().t(), t.cpu(), k)
+    for g, x in zip(got[:3], want[:3]):
+        near(g, x)
+    if k:
+        assert torch.equal(got[3].long(), want[3])
+        near(got[4], want[4])
+
+
+def off_by(h, w, steps):
+    """How far a logit may be off: ``steps`` additions, each cut off at a unit (2^-23) of a sum that no partial sum exceeds."""
+    return steps * 2.0 ** -23 * float((h.abs() @ w.abs().t()).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,H,V,scale,cap", [(3, 4096, 9000, 1.0, None), (130, 2048, 6000, 0.5, None), (64, 1024, 5001, 1.0, 30.0), (260, 776, 3000, 2.0, 5.0),
+                                             (20, 100, 900, -1.5, 8.0), (70, 33, 500, 1.0, None)])
+def test_head_rounded_logits(n, H, V, scale, cap, dtype):
+    """Sums in parts of 512 values: 32 steps of 16 and the parts; float32 sums, and bfloat16 ones of widths that no tensor map takes, value by value.
+    The logits' errors reach a log probability at most twice (its own, the sum's), an entropy at most 2 ln V times; a cap shrinks them, tanh
+    itself is off by 2^-22 of the cap."""
+    g = torch.Generator().manual_seed(n)
+    h, w = torch.randn(n, H, generator=g).to(dtype).to(DEV), (0.05 * torch.randn(V, H, generator=g)).to(dtype).to(DEV)
+    t = some_tokens(n, V, n)
+    x = h.double().cpu() @ w.double().cpu().t() * scale
+    off = abs(scale) * off_by(h.double().cpu(), w.double().cpu(), H if dtype == torch.float32 or H % 8 else min(H, 512) / 16 + H / 512)
+    if cap is not None:
+        x, off = cap * torch.tanh(x / cap), off + cap * 2.0 ** -22
+    want = plain(x, t.cpu(), 4)
+    got = head(h, w, t, 4, scale, cap)
+    tol = 2e-5 + off * (2 + 2 * math.log(V))
+    for a, b in zip(got[:3], want[:3]):
+        near(a, b, tol)
+    near(got[4], want[4], tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_head_strided_operands_and_neighbours_left_alone(dtype):
+    from airun_b200.kernels import ops
+    h, w = grid_inputs(150, 128, 3000, dtype, 4)
+    hb, wb = torch.full((150, 144), 50.0, dtype=dtype, device=DEV), torch.full((3000, 136), 50.0, dtype=dtype, device=DEV)
+    hb[:, 8:136], wb[:, :128] = h, w
+    t = some_tokens(150, 3000, 5)
+    want = plain(h.double().cpu() @ w.double().cpu().t(), t.cpu(), 5)
+    lp, ids, tops = torch.full((160,), 7.0, device=DEV), torch.full((160, 5), -7, dtype=torch.int32, device=DEV), torch.full((160, 5), 7.0, device=DEV)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ops.head_logprobs(hb[:, 8:136], wb[:, :128], t, lp[:150], err, top_ids=ids[:150], top_logprobs=tops[:150])
+    near(lp[:150].cpu(), want[0])
+    assert torch.equal(ids[:150].cpu().long(), want[3]) and int(err.item()) == 0
+    assert lp[150:].unique().tolist() == [7.0] and ids[150:].unique().tolist() == [-7] and tops[150:].unique().tolist() == [7.0]
+    ops.head_logprobs(h[:0], w, t[:0], lp[:0], err)     # no rows: nothing happens
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [4, 140])
+def test_head_rows_that_are_not_finite(n):
+    """A hidden row of NaN, and weights that give -inf or NaN logits for some tokens."""
+    h, w = grid_inputs(n, 64, 900, torch.bfloat16, 9)
+    h[:, 0] = 1.0
+    h[1] = math.nan
+    w[100:900, 0] = -math.inf
+    w[7, 3] = math.nan
+    x = h.double().cpu() @ w.double().cpu().t()
+    t = torch.full((n,), 5, dtype=torch.int32, device=DEV)
+    for k in (3, 16, 100):
+        want, got = plain(x, t.cpu(), k), head(h, w, t, k)
+        for a, b in zip(got[:3], want[:3]):
+            near(a, b)
+        assert torch.equal(got[3].long(), want[3])
+    w[100:900, 0] = math.inf
+    w[7, 3] = 0.0
+    got = head(h, w, t, 3)
+    assert got[0][0] == -math.inf and math.isnan(got[1][0]) and got[2][0] == math.inf and got[3][0, 0] == 100
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,V,k", [(4, 6000, 5), (300, 6000, 2), (3, 500, 40)])
+def test_head_on_another_stream_and_in_two_graphs(n, V, k):
+    from airun_b200.engine.batch import Workspace
+    from airun_b200.kernels import ops
+    h, w = grid_inputs(n, 256, V, torch.bfloat16, 2)
+    t = some_tokens(n, V, 2)
+    want = head(h, w, t, k)
+    places, graphs = [], []
+    for _ in range(2):
+        places.append((torch.empty(n, device=DEV), torch.empty(n, k, dtype=torch.int32, device=DEV), torch.empty(n, k, device=DEV),
+                       torch.zeros(1, dtype=torch.int32, device=DEV), Workspace(torch.device(DEV), 1 << 20)))
+    for lp, ids, tops, err, ws in places:
+        for captured in (False, True):
+            ws.reset()
+            if not captured:
+                ops.head_logprobs(h, w, t, lp, err, top_ids=ids, top_logprobs=tops, ws=ws)
+                torch.cuda.synchronize()
+                lp.fill_(7.0)
+                torch.cuda.synchronize()
+                continue
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                ops.head_logprobs(h, w, t, lp, err, top_ids=ids, top_logprobs=tops, ws=ws)
+            graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for lp, ids, tops, err, _ in places:
+        assert torch.equal(lp.cpu(), want[0]) and torch.equal(ids.cpu(), want[3]) and torch.equal(tops.cpu(), want[4]) and int(err.item()) == 0
+
+
 class _Fake:
     """A tensor's stand-in that says it is on the GPU, for the checks that come before any launch."""
 
@@ -237,3 +383,28 @@ def test_refusals(monkeypatch):
     refused("int32", rows=_Fake(5, dtype=torch.int32))
     monkeypatch.setattr(ops, "_fn", lambda *a, **k: (lambda *b: 0))
     refused("dtype", logits=_Fake(4, 100, dtype=torch.float16))
+
+
+def test_head_refusals(monkeypatch):
+    from airun_b200.kernels import ops
+    monkeypatch.setattr(ops, "_fn", lambda *a, **k: pytest.fail("launched"))
+    monkeypatch.setattr(ops, "_one_device", lambda *a: None)
+    h, w, t, lp, err = _Fake(4, 64), _Fake(100, 64), _Fake(4, dtype=torch.int32), _Fake(4), _Fake(1, dtype=torch.int32)
+
+    def refused(match, hidden=h, weight=w, tokens=t, logprob=lp, err=err, **kw):
+        with pytest.raises(ops.KernelError, match=match):
+            ops.head_logprobs(hidden, weight, tokens, logprob, err, **kw)
+
+    refused("GPU", hidden=torch.empty(4, 64))
+    refused("do not agree", weight=_Fake(100, 72))
+    refused("share a type", weight=_Fake(100, 64, dtype=torch.bfloat16))
+    refused("row-major", hidden=_Fake(64, 4).t())
+    refused("token for every row", tokens=_Fake(3, dtype=torch.int32))
+    refused("int32", tokens=_Fake(4, dtype=torch.int64))
+    refused("float32", logprob=_Fake(4, 1))
+    refused("together", top_logprobs=_Fake(4, 3))
+    refused("to the vocabulary", top_ids=_Fake(4, 101, dtype=torch.int32), top_logprobs=_Fake(4, 101))
+    refused("int32", err=_Fake(1))
+    refused("finite", scale=float("nan"))
+    refused("positive", soft_cap=0.0)
+    refused("dtype", hidden=_Fake(4, 64, dtype=torch.float16), weight=_Fake(100, 64, dtype=torch.float16))
