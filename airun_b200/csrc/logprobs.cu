@@ -5,40 +5,107 @@
 //   logprob = (x[token] - m) - ln s,  lse = m + ln s,  entropy = -sum p ln p = ln s - u / s,
 // and the k largest logits, the first id first among equals, as (x - m) - ln s.  All three sums are kept over any part of a
 // row in one pass, the maximum as it is so far; two parts join as
-//   m = max(m1, m2),  f_i = exp(m_i - m),  s = sum f_i s_i,  u = sum f_i (u_i + (m_i - m) s_i).
+//   m = max(m1, m2),  d_i = m_i - m,  f_i = exp(d_i),  s = sum f_i s_i,  u = sum f_i (u_i + d_i s_i).
 // A row with nothing above minus infinity has no distribution: its log probabilities are minus infinity, its entropy is 0.
 // A row with plus infinity has entropy NaN and log probabilities x - inf.  A token outside the vocabulary has minus infinity.
 //
 // The reference takes the same numbers from whole rows on the host (crates/airun-core/src/sample.rs:128-140, :489-503).
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 typedef unsigned long long u64;
 
 #define TOP_MAX 128
 
 // ------------------------------------------------------------------ parts of a row
+#define LOWEST (-200.0f)               // exp is 0 from here on, and so is a term's part in u
+
 struct Part { float m, s, u; };
 
+__device__ __forceinline__ float exp_of(float d) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * 1.4426950408889634f));
+    return e;
+}
+// x - m, bounded below: minus infinity, what is not a number and the difference of two equal infinities become terms of 0.
+__device__ __forceinline__ float below(float x, float m) { return fmaxf(x - m, LOWEST); }
+
 __device__ __forceinline__ Part join(const Part& a, const Part& b) {
-    const float m = fmaxf(a.m, b.m);
-    // (both empty: the differences are not numbers, and the bound makes them terms of zero)
-    const float da = fmaxf(a.m - m, -200.0f), db = fmaxf(b.m - m, -200.0f), fa = __expf(da), fb = __expf(db);
+    const float m = fmaxf(a.m, b.m), da = below(a.m, m), db = below(b.m, m), fa = exp_of(da), fb = exp_of(db);
     return {m, fa * a.s + fb * b.s, fa * fmaf(da, a.s, a.u) + fb * fmaf(db, b.s, b.u)};
 }
 
-// A part whose maximum so far becomes `m`, larger than before.
-__device__ __forceinline__ void raise_max(Part& p, float m) {
-    const float d = fmaxf(p.m - m, -200.0f), f = __expf(d);
-    p.u = f * fmaf(d, p.s, p.u);
-    p.s *= f;
-    p.m = m;
+// A part that grows, chunk by chunk.  A chunk's sums start at zero and join the others with what the additions before have rounded
+// away (compensated summation, W. Kahan, Communications of the ACM 8, 1965): beside one leading token, 8,000 terms of 1e-6 added one by one
+// are off by 3e-6, as much as the logits of a head of 4,096 values.
+struct Run {
+    float m = -INFINITY, s = 0.0f, u = 0.0f, s_lost = 0.0f, u_lost = 0.0f;
+    __device__ __forceinline__ Part part() const { return {m, s, u}; }
+};
+
+__device__ __forceinline__ void add_to(float& sum, float& lost, float x) {
+    const float y = __fsub_rn(x, lost), t = __fadd_rn(sum, y);
+    lost = __fsub_rn(__fsub_rn(t, sum), y);
+    sum = t;
 }
 
-// One logit below or at the maximum so far.  Minus infinity, NaN and what is 200 below the maximum add exp(-200) = 0.
-__device__ __forceinline__ void add_logit(Part& p, float x) {
-    const float d = fmaxf(x - p.m, -200.0f), e = __expf(d);
-    p.s += e;
-    p.u = fmaf(e, d, p.u);
+__device__ __forceinline__ u64 pair_of(float a, float b) {
+    u64 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void of_pair(u64 r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ u64 add_pair(u64 a, u64 b) {
+    u64 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ u64 fma_pair(u64 a, u64 b, u64 c) {
+    u64 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ u64 mul_pair(u64 a, u64 b) {
+    u64 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// N logits, of which none is larger than `most`.  Two at a time: additions and products take half the issue slots that way.
+template <int N> __device__ __forceinline__ void add_chunk(Run& r, const float (&x)[N], float most) {
+    if (most > r.m) {
+        const float d = below(r.m, most), f = exp_of(d);
+        r.u = f * fmaf(d, r.s, r.u);
+        r.u_lost = f * fmaf(d, r.s_lost, r.u_lost);
+        r.s *= f;
+        r.s_lost *= f;
+        r.m = most;
+    }
+    const u64 minus_m = pair_of(-r.m, -r.m), log2_e = pair_of(1.4426950408889634f, 1.4426950408889634f);
+    u64 s = 0, u = 0;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        float a, b, ea, eb;
+        of_pair(add_pair(pair_of(x[i], x[i + 1]), minus_m), a, b);
+        const u64 d = pair_of(fmaxf(a, LOWEST), fmaxf(b, LOWEST));
+        of_pair(mul_pair(d, log2_e), a, b);
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(ea) : "f"(a));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(eb) : "f"(b));
+        const u64 e = pair_of(ea, eb);
+        s = add_pair(s, e);
+        u = fma_pair(e, d, u);
+    }
+    float a, b;
+    of_pair(s, a, b);
+    add_to(r.s, r.s_lost, a + b);
+    of_pair(u, a, b);
+    add_to(r.u, r.u_lost, a + b);
+}
+
+template <int N> __device__ __forceinline__ float most_of(const float (&x)[N]) {
+    float most = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) most = fmaxf(most, x[i]);
+    return most == most ? most : -INFINITY;                        // (all of them not numbers)
 }
 
 __device__ __forceinline__ Part warp_join(Part p) {
@@ -48,7 +115,7 @@ __device__ __forceinline__ Part warp_join(Part p) {
     return p;
 }
 
-// The joined part of the block's threads, in thread 0's warp.  `sh` holds one Part a warp.
+// The joined part of the block's threads, in its first warp.  `sh` holds one Part a warp.
 template <int NT> __device__ __forceinline__ Part block_join(Part p, Part* sh) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     p = warp_join(p);
@@ -59,10 +126,18 @@ template <int NT> __device__ __forceinline__ Part block_join(Part p, Part* sh) {
     return p;
 }
 
-__device__ __forceinline__ float log_prob(const Part& p, float ln_s, float x) {
-    if (!(x > -INFINITY) || p.m == -INFINITY) return -INFINITY;
-    return p.m == INFINITY ? x - p.m : (x - p.m) - ln_s;
+// What is left of a whole row's part: the maximum, ln sum exp(x - m), the entropy.
+struct Row { float m, ln_s, entropy; };
+__device__ __forceinline__ Row row_of(const Part& p) {
+    if (p.m == -INFINITY) return {p.m, -INFINITY, 0.0f};
+    if (p.m == INFINITY) return {p.m, 0.0f, __int_as_float(0x7fffffff)};
+    const float ln_s = logf(p.s);
+    return {p.m, ln_s, ln_s - p.u / p.s};
 }
+__device__ __forceinline__ float log_prob(const Row& r, float x) {
+    return x > -INFINITY && r.m > -INFINITY ? (x - r.m) - r.ln_s : -INFINITY;
+}
+__device__ __forceinline__ float row_lse(const Row& r) { return fabsf(r.m) < INFINITY ? r.m + r.ln_s : r.m; }
 
 // ------------------------------------------------------------------ the k largest of many
 // A logit and its id as one number: larger logits first, among equals the lower id first; 0 is no logit.  -0 counts as 0.
@@ -195,11 +270,13 @@ template <typename T> struct Pack;
 template <> struct Pack<float> {
     static constexpr int N = 4;
     float4 v;
+    __device__ __forceinline__ void nothing() { v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY); }
     __device__ __forceinline__ float at(int i) const { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 };
 template <> struct Pack<__nv_bfloat16> {
     static constexpr int N = 8;
     uint4 v;
+    __device__ __forceinline__ void nothing() { v = make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u); }      // minus infinities
     __device__ __forceinline__ float at(int i) const {
         const unsigned w = i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w;
         return __uint_as_float((i & 1) ? (w & 0xFFFF0000u) : (w << 16));
@@ -216,6 +293,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(const TokenParams p,
     __shared__ TopShared<NT> top;
     __shared__ Part s_parts[32];
     __shared__ Part s_mine;
+    __shared__ Row s_row;
     const int tid = threadIdx.x;
     const int part = CLUSTER ? (int)cluster_rank() : 0, parts = CLUSTER ? n_parts : 1;
     const int r = CLUSTER ? blockIdx.x / parts : blockIdx.x;
@@ -236,43 +314,37 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(const TokenParams p,
     // the element ahead of the vectors that is this thread's, and the one behind them
     const int ahead = part == 0 && tid < lead ? tid : -1, behind = part == parts - 1 && tid < V - tail ? tail + tid : -1;
 
-    Part mine = {-INFINITY, 0.0f, 0.0f};
+    Run mine;
     float second = -INFINITY;                                    // largest of the batches but the one with the maximum
     int best_batch = -1;
     if (ahead >= 0) {
-        const float x = to_f32<T>(row[ahead]);
-        if (x > mine.m) mine.m = x;
-        add_logit(mine, x);
+        const float x[2] = {to_f32<T>(row[ahead]), -INFINITY};
+        add_chunk(mine, x, most_of(x));
         second = mine.m;                                         // (its own key is looked at below)
     }
     for (int b = 0; b < n_batches; ++b) {
-        Pack<T> x[U];
+        Pack<T> in[U];
         const int first = v0 + b * U * NT + tid;
 #pragma unroll
-        for (int i = 0; i < U; ++i) if (first + i * NT < v1) x[i] = from[first + i * NT];
-        float most = -INFINITY;
+        for (int i = 0; i < U; ++i) {
+            if (first + i * NT < v1) in[i] = from[first + i * NT];
+            else in[i].nothing();
+        }
+        float x[U * VEC];
 #pragma unroll
-        for (int i = 0; i < U; ++i)
-            if (first + i * NT < v1)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) most = fmaxf(most, x[i].at(j));
+        for (int i = 0; i < U * VEC; ++i) x[i] = in[i / VEC].at(i % VEC);
+        const float most = most_of(x);
         if (most > mine.m) {
             if (best_batch >= 0) second = mine.m;
-            raise_max(mine, most);
             best_batch = b;
         } else {
             second = fmaxf(second, most);
         }
-#pragma unroll
-        for (int i = 0; i < U; ++i)
-            if (first + i * NT < v1)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) add_logit(mine, x[i].at(j));
+        add_chunk(mine, x, most);
     }
     if (behind >= 0) {
-        const float x = to_f32<T>(row[behind]);
-        if (x > mine.m) raise_max(mine, x);
-        add_logit(mine, x);
+        const float x[2] = {to_f32<T>(row[behind]), -INFINITY};
+        add_chunk(mine, x, most_of(x));
     }
 
     if (p.k > 0) {
@@ -306,7 +378,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(const TokenParams p,
             if (behind >= 0) f(key_of(to_f32<T>(row[behind]), behind));
         });
     }
-    Part all = block_join<NT>(mine, s_parts);
+    Part all = block_join<NT>(mine.part(), s_parts);
     if (CLUSTER) {
         if (tid == 0) s_mine = all;
         cluster_sync_all();
@@ -345,19 +417,19 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(const TokenParams p,
         if (part != 0) return;
     }
     if (tid == 0) {
-        const float ln_s = logf(all.s);
-        s_mine = {all.m, ln_s, 0.0f};
-        p.logprob[r] = log_prob(all, ln_s, given);
-        if (p.lse) p.lse[r] = fabsf(all.m) < INFINITY ? all.m + ln_s : all.m;
-        if (p.entropy) p.entropy[r] = all.m == -INFINITY ? 0.0f : all.m == INFINITY ? __int_as_float(0x7fffffff) : ln_s - all.u / all.s;
+        const Row w = row_of(all);
+        s_row = w;
+        p.logprob[r] = log_prob(w, given);
+        if (p.lse) p.lse[r] = row_lse(w);
+        if (p.entropy) p.entropy[r] = w.entropy;
     }
     if (p.k > 0) {
         __syncthreads();
-        const Part q = {s_mine.m, 0.0f, 0.0f};
+        const Row w = s_row;
         for (int i = tid; i < p.k; i += NT) {
             const u64 key = top.top[i];
             p.top_ids[(size_t)r * p.k + i] = key ? key_id(key) : -1;
-            p.top_logprobs[(size_t)r * p.k + i] = key ? log_prob(q, s_mine.s, key_logit(key)) : -INFINITY;
+            p.top_logprobs[(size_t)r * p.k + i] = key ? log_prob(w, key_logit(key)) : -INFINITY;
         }
     }
 }
@@ -389,4 +461,443 @@ AIRUN_EXPORT int airun_token_logprobs(const void* logits, int dtype, long long l
     if (dtype == AIRUN_DT_F32) return V <= 2048 ? launch_tokens<float, 128>(p, n, 1, stream) : launch_tokens<float, 512>(p, n, parts, stream);
     if (dtype == AIRUN_DT_BF16) return V <= 2048 ? launch_tokens<__nv_bfloat16, 128>(p, n, 1, stream) : launch_tokens<__nv_bfloat16, 512>(p, n, parts, stream);
     return AIRUN_ERR_UNSUPPORTED;
+}
+
+// ------------------------------------------------------------------ from hidden states
+// The logits of a row are its product with the head's weight [V][K].  They are formed in tensor memory, a tile of rows x `bn` ids at a
+// time, and every thread of the epilogue keeps the three sums, the given token's logit and a list of the k largest for one row:
+// its lane of tensor memory is that row, its ids those of half of the tiles' columns.  The vocabulary is cut into `splits` ranges of
+// `tiles` tiles; a block (a pair) walks the tiles of one range for one block of rows, then the parts of each row are joined by
+// head_join_kernel.  Neither logits nor anything of their size is written.
+//   PAIR   : two SMs to 256 rows, tcgen05.mma.cta_group::2 with M = 256; each brings 128 rows and half of the ids, 32 KB a K-step of 64
+//            values, which is what 512 clocks of products leave time for.  What prompts run on.
+//   !PAIR  : an SM to 128 rows, of which only `x_rows` are brought (what the products read behind them ends in lanes nobody looks at): up
+//            to 128 rows are bound by the weights' bytes.
+//   warp 0    : TMA loads into a ring of stages; asks for weights, which no kernel writes, ahead of the wait for the kernel in front;
+//   warp 1    : allocates tensor memory, issues the products (in a pair, the leader's);
+//   warps 4-11: epilogue, two warps a quadrant of lanes, every other 32 ids of a tile; they take the registers of the first four.
+// The tensor cores cut a running sum off where float32 rounds, so its error grows with the products in it.  A buffer of tensor memory holds
+// `part` K-steps; the epilogue adds the parts up in registers, rounded, 128 sums a thread, while the other buffer fills.
+#define HEAD_THREADS 384
+#define HEAD_LANES 256                                             // threads of the epilogue
+#define HEAD_TOP 16                                                // longest list: 32 KB
+#define HEAD_SMEM 230400                                           // stages, lists and 1 KB to align them
+#define HEAD_STAGES 12                                             // at most
+#define HEAD_REGS 168                                              // a thread at launch: 384 x 168 = 128 x 40 + 256 x 232
+#define BK 64
+
+struct HeadParams {
+    int n, V, K;
+    int row_blocks, splits, tiles, bn, part;
+    int x_rows, stages, list_at;                                   // rows a stage brings; stages; where the lists begin in shared memory
+    const int32_t* tokens;
+    float scale, cap;
+    int k;
+    float* stats;                                                  // [3][2 splits][n]: m, s, u
+    float* given;                                                  // [n] logits of the given tokens
+    u64* keys;                                                     // [n][2 splits][k]
+    int* err;
+};
+
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void umma_bf16_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+
+// Puts a logit into a thread's list of its k largest, in shared memory, HEAD_LANES entries from one to the next: the largest first, equal
+// ones in the order they come, which is that of their ids.  Four entries at a time, so that their loads are one latency.
+__device__ __forceinline__ void list_insert(float2* list, int k, float2 x) {
+    bool found = false;
+    for (int at = 0; at < k; at += 4) {
+        float2 e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = at + i < k ? list[(at + i) * HEAD_LANES] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            found |= x.x > e[i].x;
+            if (found) {
+                const float2 t = e[i];
+                if (at + i < k) list[(at + i) * HEAD_LANES] = x;
+                x = t;
+            }
+        }
+    }
+}
+
+template <bool PAIR, bool CAP>
+__global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
+    const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const HeadParams p) {
+    pdl_trigger();
+    constexpr int CTAS = PAIR ? 2 : 1;
+    __shared__ __align__(8) uint64_t bars[2 * HEAD_STAGES + 4];    // full (a pair: the leader's), empty of the stages; full, empty (the leader's) of the sums
+    __shared__ uint32_t tmem_slot;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+    const int rank = PAIR ? (int)cluster_rank() : 0, group = PAIR ? blockIdx.x >> 1 : blockIdx.x, groups = PAIR ? gridDim.x >> 1 : gridDim.x;
+    const int kb_total = (p.K + BK - 1) / BK, units = p.row_blocks * p.splits, range = p.tiles * p.bn;
+    const int w_rows = p.bn / CTAS, w_bytes = w_rows * (BK * 2), x_bytes = p.x_rows * (BK * 2), stages = p.stages;
+    // the stages' weights, then their rows
+    const uint32_t w_at = smem_u32(smem), x_at = w_at + stages * w_bytes;
+    const uint32_t full = smem_u32(bars), empty = full + 8 * HEAD_STAGES, accf = empty + 8 * HEAD_STAGES, acce = accf + 16;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < HEAD_STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(accf + 8 * b, 1); mbar_init(acce + 8 * b, 8 * CTAS); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            tmem_alloc(smem_u32(&tmem_slot), 512);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (PAIR) cluster_sync_all();                        // the leader's barriers are there before anything arrives at them
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const uint32_t full_lead = PAIR ? map_to_cta(full, 0) : full, acce_lead = PAIR ? map_to_cta(acce, 0) : acce;
+
+    struct Unit { int x0, w0, w_end; };                            // first row of this CTA; ids
+    auto unit_of = [&](int u) {
+        const int w0 = u / p.row_blocks * range;
+        return Unit{u % p.row_blocks * (128 * CTAS) + rank * 128, w0, min(p.V, w0 + range)};
+    };
+    const uint32_t bytes = CTAS * (x_bytes + w_bytes);
+    auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar, int x, int y) {
+        if constexpr (PAIR) tma_load_2d_pair(dst, map, bar, x, y);
+        else tma_load_2d(dst, map, bar, x, y);
+    };
+    const int first_n = group < units ? min(kb_total, stages) : 0;
+    if (warp == 0 && elect_one()) {
+        for (int i = 0; i < first_n; ++i) {
+            if (rank == 0) mbar_expect_tx(full + 8 * i, bytes);
+            load(&map_w, w_at + i * w_bytes, full_lead + 8 * i, i * BK, unit_of(group).w0 + rank * w_rows);
+        }
+    }
+    pdl_wait();
+
+    bool ok = true;
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        int it = 0, s = 0;                                         // K-steps so far, and their place in the ring
+        uint32_t phase = 0;                                        // of the ring's barriers, one round after the other
+        if (warp == 0) {
+            for (int u = group; u < units && ok; u += groups) {
+                const Unit t = unit_of(u);
+                for (int w0 = t.w0; w0 < t.w_end && ok; w0 += p.bn) {
+                    for (int kb = 0; kb < kb_total; ++kb, ++it) {
+                        if (it >= first_n && !mbar_wait_warp(empty + 8 * s, phase ^ 1)) { ok = false; break; }
+                        const uint32_t bar = full_lead + 8 * s;
+                        if (elect_one()) {
+                            if (it >= first_n) {
+                                if (rank == 0) mbar_expect_tx(full + 8 * s, bytes);
+                                load(&map_w, w_at + s * w_bytes, bar, kb * BK, w0 + rank * w_rows);
+                            }
+                            load(&map_x, x_at + s * x_bytes, bar, kb * BK, t.x0);
+                        }
+                        __syncwarp();
+                        if (++s == stages) { s = 0; phase ^= 1; }
+                    }
+                }
+            }
+            // the last commits arrive at this CTA's barriers before it may leave
+            for (int i = max(0, it - stages); i < it && ok; ++i)
+                ok = mbar_wait_warp(empty + 8 * (i % stages), (i / stages) & 1);
+            if (!ok) atomicOr(p.err, AIRUN_DEV_TIMEOUT);
+        } else if (warp == 1 && rank == 0) {
+            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(128 * CTAS >> 4) << 24);
+            int n = 0;                                             // sums so far
+            auto sum_up = [&](int first, int end) {
+                const int buf = n & 1;
+                if (!mbar_wait_warp(acce + 8 * buf, ((n >> 1) & 1) ^ 1)) { ok = false; return; }
+                tc_fence_after();
+                for (int kb = first; kb < end; ++kb) {
+                    if (!mbar_wait_warp(full + 8 * s, phase)) { ok = false; return; }
+                    tc_fence_after();
+                    const uint64_t da = smem_desc_sw128(x_at + s * x_bytes), db = smem_desc_sw128(w_at + s * w_bytes);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < BK / 16; ++k) {
+                            const uint32_t more = (kb > first || k > 0) ? 1u : 0u;
+                            if constexpr (PAIR) umma_bf16_pair(tmem + buf * 256, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), idesc, more);
+                            else umma_bf16(tmem + buf * 256, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), idesc, more);
+                        }
+                        if constexpr (PAIR) {
+                            umma_commit_pair(empty + 8 * s);
+                            if (kb + 1 == end) umma_commit_pair(accf + 8 * buf);
+                        } else {
+                            umma_commit(empty + 8 * s);
+                            if (kb + 1 == end) umma_commit(accf + 8 * buf);
+                        }
+                    }
+                    __syncwarp();
+                    if (++s == stages) { s = 0; phase ^= 1; }
+                }
+                ++n;
+            };
+            for (int u = group; u < units && ok; u += groups) {
+                const Unit t = unit_of(u);
+                for (int w0 = t.w0; w0 < t.w_end && ok; w0 += p.bn)
+                    for (int first = 0; first < kb_total && ok; first += p.part) sum_up(first, min(first + p.part, kb_total));
+            }
+            if (!ok) atomicOr(p.err, AIRUN_DEV_TIMEOUT);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        const int quad = warp & 3, half = (warp - 4) >> 2;
+        float2* list = reinterpret_cast<float2*>(smem + p.list_at) + (threadIdx.x - 128);
+        int n = 0;                                                 // sums so far
+        for (int u = group; u < units && ok; u += groups) {
+            const Unit t = unit_of(u);
+            const int row = t.x0 + quad * 32 + lane;
+            const bool row_on = row < p.n, warp_on = t.x0 + quad * 32 < p.n;
+            const int token = row_on ? p.tokens[row] : -1;
+            Run mine;
+            float least = row_on && p.k > 0 ? -INFINITY : INFINITY;              // of the list
+            for (int i = 0; i < p.k; ++i) list[i * HEAD_LANES] = make_float2(-INFINITY, __int_as_float(-1));
+            for (int w0 = t.w0; w0 < t.w_end && ok; w0 += p.bn) {
+                float acc[4][32];                                  // ids 32 half + 64 j and 31 more
+                for (int kb = 0; kb < kb_total; kb += p.part, ++n) {
+                    const int buf = n & 1;
+                    ok = mbar_wait(accf + 8 * buf, (n >> 1) & 1);
+                    if (!ok) { atomicOr(p.err, AIRUN_DEV_TIMEOUT); break; }
+                    tc_fence_after();
+                    __syncwarp();
+                    if (warp_on) {
+                        // (a load takes 1,100 clocks while products run, four at once 1,900, so as many as registers are free for are on their
+                        // way together.  What lies beyond the tile's ids, but inside the buffer, is read and not looked at.)
+                        const uint32_t lanes = tmem + buf * 256 + ((uint32_t)(quad * 32) << 16) + 32 * half;
+                        if (kb == 0) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) tmem_ld32_async(lanes + 64 * j, reinterpret_cast<uint32_t*>(acc[j]));
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) tmem_wait32(reinterpret_cast<uint32_t*>(acc[j]));
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; j += 2) {
+                                uint32_t a[32], b[32];
+                                tmem_ld32_async(lanes + 64 * j, a);
+                                tmem_ld32_async(lanes + 64 * j + 64, b);
+                                tmem_wait32(a);
+                                tmem_wait32(b);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) {
+                                    acc[j][i] += __uint_as_float(a[i]);
+                                    acc[j + 1][i] += __uint_as_float(b[i]);
+                                }
+                            }
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if constexpr (PAIR) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(acce_lead + 8 * buf) : "memory");
+                        else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(acce + 8 * buf) : "memory");
+                    }
+                }
+                if (!ok) break;
+                if (!warp_on) continue;
+                const int ids = min(p.bn, t.w_end - w0);           // of this tile
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int c = 32 * half + 64 * j, first = w0 + c;
+                    if (c >= ids) break;
+                    float (&v)[32] = acc[j];
+                    if (c + 32 > ids) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = c + i < ids ? v[i] : __int_as_float(0x7fffffff);       // no number: nowhere counted
+                    }
+                    if (CAP || p.scale != 1.0f) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] *= p.scale;
+                    }
+                    if (CAP) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = p.cap * tanhf(v[i] / p.cap);
+                    }
+                    if (token >= first && token < min(first + 32, t.w_end)) {
+                        float x = v[0];
+#pragma unroll
+                        for (int i = 1; i < 32; ++i) x = token == first + i ? v[i] : x;
+                        p.given[row] = x;
+                    }
+                    const float most = most_of(v);
+                    add_chunk(mine, v, most);
+                    if (__any_sync(0xffffffffu, most > least)) {
+                        uint32_t larger = 0;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) larger |= v[i] > least ? 1u << i : 0u;
+                        while (__any_sync(0xffffffffu, larger != 0)) {
+                            const int i = larger ? __ffs(larger) - 1 : 0;
+                            float x[16];
+#pragma unroll
+                            for (int a = 0; a < 16; ++a) x[a] = i & 1 ? v[2 * a + 1] : v[2 * a];
+#pragma unroll
+                            for (int b = 1; b < 5; ++b)
+#pragma unroll
+                                for (int a = 0; a < (16 >> b); ++a) x[a] = (i >> b) & 1 ? x[2 * a + 1] : x[2 * a];
+                            if (larger && x[0] > least) {
+                                list_insert(list, p.k, make_float2(x[0], __int_as_float(first + i)));
+                                least = list[(p.k - 1) * HEAD_LANES].x;
+                            }
+                            larger &= larger - 1;
+                        }
+                    }
+                }
+            }
+            if (row_on) {
+                const int parts = 2 * p.splits, part = 2 * (u / p.row_blocks) + half;
+                float* to = p.stats + (size_t)part * p.n + row;
+                to[0] = mine.m;
+                to[(size_t)parts * p.n] = mine.s;
+                to[(size_t)2 * parts * p.n] = mine.u;
+                u64* keys = p.keys + ((size_t)row * parts + part) * p.k;
+                for (int i = 0; i < p.k; ++i) {
+                    const float2 e = list[i * HEAD_LANES];
+                    const int id = __float_as_int(e.y);
+                    keys[i] = id < 0 ? 0 : key_of(e.x, id);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (PAIR) cluster_sync_all();                        // neither CTA leaves, or frees, while the other works on both
+    if (warp == 1) {
+        tc_fence_after();
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        else tmem_dealloc(tmem, 512);
+    }
+}
+
+// The parts of a row become its results: a block a row.  What is in no list is minus infinity (or not a number, which counts as that): where the lists
+// hold fewer than k, the lowest ids that are in none follow.
+#define JOIN_THREADS 128
+__global__ __launch_bounds__(JOIN_THREADS) void head_join_kernel(
+    const float* stats, const float* given, const u64* keys, const int32_t* tokens, int n, int V, int parts, int k,
+    float* logprob, float* entropy, float* lse, int32_t* top_ids, float* top_logprobs) {
+    pdl_trigger();
+    __shared__ TopShared<JOIN_THREADS> top;
+    __shared__ Part s_parts[JOIN_THREADS / 32];
+    __shared__ Row s_row;
+    const int r = blockIdx.x, tid = threadIdx.x;
+    pdl_wait();
+    Part mine = {-INFINITY, 0.0f, 0.0f};
+    for (int i = tid; i < parts; i += JOIN_THREADS) {
+        const float* at = stats + (size_t)i * n + r;
+        mine = join(mine, Part{at[0], at[(size_t)parts * n], at[(size_t)2 * parts * n]});
+    }
+    if (k > 0) {
+        const u64* mine_k = keys + (size_t)r * parts * k;
+        u64 best = 0;
+        for (int i = tid; i < parts * k; i += JOIN_THREADS) best = mine_k[i] > best ? mine_k[i] : best;
+        select_top<JOIN_THREADS>(top, best, k, [&](u64, auto f) {
+            for (int i = tid; i < parts * k; i += JOIN_THREADS) if (mine_k[i]) f(mine_k[i]);
+        });
+        if (tid == 0) {
+            int at = 0, id = 0;
+            while (at < k && top.top[at]) ++at;
+            for (const int found = at; at < k; ++at, ++id) {
+                for (int j = 0; j < found; ++j) if (key_id(top.top[j]) == id) { ++id; j = -1; }
+                top.top[at] = key_of(-INFINITY, id);
+            }
+        }
+    }
+    const Part all = block_join<JOIN_THREADS>(mine, s_parts);
+    if (tid == 0) {
+        const Row w = row_of(all);
+        const int token = tokens[r];
+        s_row = w;
+        logprob[r] = token >= 0 && token < V ? log_prob(w, given[r]) : -INFINITY;
+        if (lse) lse[r] = row_lse(w);
+        if (entropy) entropy[r] = w.entropy;
+    }
+    __syncthreads();
+    const Row w = s_row;
+    for (int i = tid; i < k; i += JOIN_THREADS) {
+        const u64 key = top.top[i];
+        top_ids[(size_t)r * k + i] = key_id(key);
+        top_logprobs[(size_t)r * k + i] = log_prob(w, key_logit(key));
+    }
+}
+
+// A tensor map of a row-major [rows][K] bfloat16 matrix with boxes of box_rows x 64.
+static int head_map(CUtensorMap* out, const void* ptr, long long rows, long long K, long long ld, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return AIRUN_ERR_UNSUPPORTED;
+    cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    cuuint32_t box[2] = {BK, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? AIRUN_OK : AIRUN_ERR_ARG;
+}
+
+template <bool PAIR, bool CAP>
+static int launch_head(const CUtensorMap& mx, const CUtensorMap& mw, HeadParams p, cudaStream_t stream) {
+    static unsigned long long configured = 0;
+    auto kern = head_logprobs_kernel<PAIR, CAP>;
+    const int w_bytes = p.bn / (PAIR ? 2 : 1) * (BK * 2), x_bytes = p.x_rows * (BK * 2);
+    // the products read 128 rows from a stage's first on, in the last one beyond what it brings
+    const int lists = p.k * HEAD_LANES * 8, beyond = 128 * BK * 2 - x_bytes;
+    p.stages = (HEAD_SMEM - 1024 - lists - beyond) / (w_bytes + x_bytes);
+    if (p.stages > HEAD_STAGES) p.stages = HEAD_STAGES;
+    p.list_at = p.stages * (w_bytes + x_bytes) + beyond;
+    const int smem = 1024 + p.list_at + lists;
+    if (first_on_device(configured)) {
+        cudaFuncAttributes at;
+        cudaError_t e = cudaFuncGetAttributes(&at, kern);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, HEAD_SMEM);
+        // the epilogue's warps would wait for good for registers that the block was not launched with
+        if (e == cudaSuccess && at.numRegs < HEAD_REGS) e = cudaErrorInvalidKernelImage;
+        if (e != cudaSuccess) { configured = 0; return (int)e; }
+    }
+    const long long units = (long long)p.row_blocks * p.splits;
+    const int most = airun_sm_count() / (PAIR ? 2 : 1);
+    const int groups = units < most ? (int)units : most;
+    if constexpr (PAIR) airun_launch_clusters(kern, dim3(2 * groups), dim3(HEAD_THREADS), smem, stream, dim3(2), mx, mw, p);
+    else airun_launch(kern, dim3(groups), dim3(HEAD_THREADS), smem, stream, mx, mw, p);
+    return AIRUN_OK;
+}
+
+// x: [n][K], W: [V][K] bfloat16, rows ldx, ldw elements apart (16-byte aligned); the vocabulary in `splits` ranges of `tiles` tiles of `bn` ids, of which
+// none is empty.  scratch: 4 (6 splits + 1) n bytes, rounded up to 16, and 16 splits n k more.
+AIRUN_EXPORT int airun_head_logprobs(const void* x, const void* W, int n, int V, int K, long long ldx, long long ldw, const int32_t* tokens,
+                                     float scale, float cap, int pair, int splits, int tiles, int bn, int part, void* scratch, float* logprob, float* entropy,
+                                     float* lse, int k, int32_t* top_ids, float* top_logprobs, int* err, cudaStream_t stream) {
+    if (n <= 0 || V <= 0 || K <= 0 || K % 8 || ldx < K || ldw < K || ldx % 8 || ldw % 8 || ((uintptr_t)x | (uintptr_t)W | (uintptr_t)scratch) & 15) return AIRUN_ERR_ARG;
+    if (!x || !W || !tokens || !scratch || !logprob || !err || k < 0 || k > HEAD_TOP || k > V || (k > 0 && (!top_ids || !top_logprobs))) return AIRUN_ERR_ARG;
+    if (bn < 16 || bn > 256 || bn % (pair ? 32 : 16) || part < 1 || tiles < 1 || splits < 1 || (long long)splits * tiles * bn < V || (long long)(splits - 1) * tiles * bn >= V) return AIRUN_ERR_ARG;
+    const int row_blocks = (n + (pair ? 255 : 127)) / (pair ? 256 : 128);
+    if ((long long)splits * tiles * bn > 0x7fff0000 || (long long)row_blocks * splits > 0x3fffffff || n > (1 << 27)) return AIRUN_ERR_ARG;
+    CUtensorMap mx, mw;
+    int r;
+    const int x_rows = pair || n > 128 ? 128 : (n + 7) / 8 * 8;
+    if ((r = head_map(&mx, x, n, K, ldx, x_rows)) != AIRUN_OK) return r;
+    if ((r = head_map(&mw, W, V, K, ldw, pair ? bn / 2 : bn)) != AIRUN_OK) return r;
+    HeadParams p = {n, V, K, row_blocks, splits, tiles, bn, part, x_rows, 0, 0, tokens, scale, cap, k, (float*)scratch, nullptr, nullptr, err};
+    p.given = p.stats + (size_t)6 * splits * n;
+    p.keys = (u64*)((uint8_t*)scratch + ((size_t)4 * (6 * (size_t)splits + 1) * n + 15) / 16 * 16);
+    if (pair) r = cap > 0.0f ? launch_head<true, true>(mx, mw, p, stream) : launch_head<true, false>(mx, mw, p, stream);
+    else r = cap > 0.0f ? launch_head<false, true>(mx, mw, p, stream) : launch_head<false, false>(mx, mw, p, stream);
+    if (r != AIRUN_OK) return r;
+    airun_launch(head_join_kernel, dim3(n), dim3(JOIN_THREADS), 0, stream, (const float*)p.stats, (const float*)p.given, (const u64*)p.keys, tokens, n, V, 2 * splits, k,
+                 logprob, entropy, lse, top_ids, top_logprobs);
+    return airun_launch_status();
 }

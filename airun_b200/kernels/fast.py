@@ -381,6 +381,61 @@ def linear_unsliced_bf16(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, er
     return True
 
 
+HEAD_TOP = 16                          # most alternatives that the fused head keeps lists for (csrc/logprobs.cu)
+
+
+@lru_cache(maxsize=4096)
+def plan_head(n: int, V: int, K: int, sms: int = B200_SMS) -> Tuple[bool, int, int, int, int]:
+    """(pairs of SMs, ranges of the vocabulary, tiles of a range, ids of a tile, K-steps of a part of a sum) for the log probabilities of n rows.
+
+    Up to 128 rows an SM to all of them, as the weights' bytes are the bound; sums in parts of 256 values cost nothing there.  Above, by the clocks of
+    the rounds that blocks of 128 rows (256 for a pair) and ranges take: 3 an id and K-step, 4 % less on pairs, whose tiles cost 2,500 more
+    where K is too short to hide them; 6,000 a range, and 2 % a round for SMs that no longer read the same weights at the same time.  B200, sustained, us,
+    pairs and single SMs: 2,048 x 4,096 1,868 and 1,957; 4,095 x 2,048 1,888 and 1,950; 2,048 x 512 309 and 240; with fewer rows
+    that are not there, 300 x 4,096 479 and 376, 640 x 2,048 386 and 294 (151,936 ids all)."""
+    kb = (K + 63) // 64
+    best = None
+    for pair in (False, True) if n > 128 else (False,):
+        rows, groups, unit = (256, sms // 2, 32) if pair else (128, sms, 16)
+        blocks = (n + rows - 1) // rows
+        for rounds in range(1, 9):
+            ranges = rounds * groups // blocks
+            if ranges < 1:
+                continue
+            per = (V + ranges - 1) // ranges
+            tiles = (per + 255) // 256
+            bn = ((per + tiles - 1) // tiles + unit - 1) // unit * unit
+            ranges = (V + tiles * bn - 1) // (tiles * bn)
+            turns = (blocks * ranges + groups - 1) // groups
+            tile = kb * bn * 2.9 + (2500 if kb < 16 else 0) if pair else kb * bn * 3.0
+            clocks = turns * (tiles * tile + 6000) * (1 + 0.02 * (turns - 1))
+            if best is None or clocks < best[0]:
+                best = clocks, pair, ranges, tiles, bn
+    if best is None:                                      # more blocks of rows than that: each walks the whole vocabulary
+        best = 0, True, 1, (V + 255) // 256, 256
+    return best[1:] + (4 if n <= 128 else 8,)
+
+
+def head_logprobs_bf16(hidden, weight, tokens, logprob, entropy, lse, top_ids, top_logprobs, scale: float, soft_cap: Optional[float], err,
+                       alloc) -> bool:
+    """``ops.head_logprobs`` in one kernel that forms the logits in tensor memory, and one that joins its parts; False where it does not take the
+    sizes.  ``alloc``: gives scratch, as a Workspace's does."""
+    n, K = hidden.shape
+    V = weight.shape[0]
+    k = 0 if top_ids is None else top_ids.shape[1]
+    if "head_logprobs" in DISABLED or not _usable(hidden, weight) or k > HEAD_TOP:
+        return False
+    pair, splits, tiles, bn, part = plan_head(n, V, K, machine(hidden.device).sms)
+    scratch = alloc(((4 * (6 * splits + 1) * n + 15) // 16 * 16 + 16 * splits * n * k,), torch.uint8)
+    f = _fn("logprobs", "airun_head_logprobs",
+            [c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_void_p, c_float, c_float, c_int, c_int, c_int, c_int, c_int, c_void_p,
+             c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p])
+    _check(f(_p(hidden), _p(weight), n, V, K, hidden.stride(0) if n > 1 else max(K, hidden.stride(0)), weight.stride(0) if V > 1 else max(K, weight.stride(0)),
+             _p(tokens), float(scale), float(soft_cap or 0.0), 1 if pair else 0, splits, tiles, bn, part, _p(scratch), _p(logprob), _p(entropy), _p(lse), k,
+             _p(top_ids), _p(top_logprobs), _p(err), _stream()), "head_logprobs")
+    return True
+
+
 def linear_swiglu_bf16(ctx, x: torch.Tensor, w_gu: torch.Tensor, out: torch.Tensor, group: int, normed=None) -> bool:
     if group != 16 or not _usable(x, w_gu) or w_gu.shape[0] % 32 != 0:
         return False

@@ -1348,6 +1348,10 @@ def head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tens
     if n == 0:
         return
     alloc = ws.alloc if ws is not None else (lambda shape, dtype: torch.empty(shape, dtype=dtype, device=hidden.device))
+    if hidden.dtype == torch.bfloat16:
+        from . import fast
+        if fast.head_logprobs_bf16(hidden, weight, tokens, logprob, entropy, lse, top_ids, top_logprobs, scale, soft_cap, err, alloc):
+            return
     step = min(n, max(1, HEAD_CHUNK // V))
     logits = alloc((step, V), torch.float32)
     for a in range(0, n, step):
