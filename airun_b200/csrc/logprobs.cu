@@ -479,9 +479,8 @@ AIRUN_EXPORT int airun_token_logprobs(const void* logits, int dtype, long long l
 // The tensor cores cut a running sum off where float32 rounds, so its error grows with the products in it.  A buffer of tensor memory holds
 // `part` K-steps; the epilogue adds the parts up in registers, rounded, 128 sums a thread, while the other buffer fills.
 #define HEAD_THREADS 384
-#define HEAD_LANES 256                                             // threads of the epilogue
-#define HEAD_TOP 16                                                // longest list: 32 KB
-#define HEAD_SMEM 230400                                           // stages, lists and 1 KB to align them
+#define HEAD_TOP 16                                                // longest list
+#define HEAD_SMEM 230400                                           // stages and 1 KB to align them
 #define HEAD_STAGES 12                                             // at most
 #define HEAD_REGS 168                                              // a thread at launch: 384 x 168 = 128 x 40 + 256 x 232
 #define BK 64
@@ -489,7 +488,7 @@ AIRUN_EXPORT int airun_token_logprobs(const void* logits, int dtype, long long l
 struct HeadParams {
     int n, V, K;
     int row_blocks, splits, tiles, bn, part;
-    int x_rows, stages, list_at;                                   // rows a stage brings; stages; where the lists begin in shared memory
+    int x_rows, stages;                                            // rows a stage brings; stages
     const int32_t* tokens;
     float scale, cap;
     int k;
@@ -515,27 +514,44 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 
-// Puts a logit into a thread's list of its k largest, in shared memory, HEAD_LANES entries from one to the next: the largest first, equal
-// ones in the order they come, which is that of their ids.  Four entries at a time, so that their loads are one latency.
-__device__ __forceinline__ void list_insert(float2* list, int k, float2 x) {
-    bool found = false;
-    for (int at = 0; at < k; at += 4) {
-        float2 e[4];
+// A thread's k <= N largest logits with their ids: the largest first, equal ones in the order they come, which is that of their ids.  In registers: while
+// products read their operands from shared memory, a load from there takes hundreds of clocks (a logit put into a list there took 1,900).
+template <int N> struct TopList {
+    float x[N];
+    int id[N];
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = at + i < k ? list[(at + i) * HEAD_LANES] : make_float2(-INFINITY, 0.0f);
+        for (int i = 0; i < N; ++i) { x[i] = -INFINITY; id[i] = -1; }
+    }
+    __device__ __forceinline__ void put(float v, int at) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            found |= x.x > e[i].x;
-            if (found) {
-                const float2 t = e[i];
-                if (at + i < k) list[(at + i) * HEAD_LANES] = x;
-                x = t;
-            }
+        for (int i = N - 1; i >= 0; --i) {
+            const bool here = v > x[i], before = i > 0 && v > x[i > 0 ? i - 1 : 0];
+            x[i] = before ? x[i > 0 ? i - 1 : 0] : here ? v : x[i];
+            id[i] = before ? id[i > 0 ? i - 1 : 0] : here ? at : id[i];
         }
     }
+    __device__ __forceinline__ float least(int k) const {
+        float v = x[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) v = k > i ? x[i] : v;
+        return v;
+    }
+};
+template <> struct TopList<0> {};
+
+// cap * tanh(x / cap).  tanh z = 1 - 2 / (e^2z + 1), off by 2^-24 or so; below 1/4, where that would be many units, the odd series to z^9
+// (the next term is below 3e-9).  Without branches: tanhf, which has some, took 60 of 134 us of 700 rows x [20000, 1024].
+__device__ __forceinline__ float capped(float x, float cap, float over_cap) {
+    const float z = x * over_cap, q = z * z;
+    const float near = fmaf(z * q, fmaf(q, fmaf(q, fmaf(q, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), z);
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * (2.0f * 1.4426950408889634f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
+    return cap * (fabsf(z) < 0.25f ? near : fmaf(-2.0f, r, 1.0f));
 }
 
-template <bool PAIR, bool CAP>
+template <bool PAIR, int TOP>
 __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
     const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const HeadParams p) {
     pdl_trigger();
@@ -660,7 +676,7 @@ __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
         const int quad = warp & 3, half = (warp - 4) >> 2;
-        float2* list = reinterpret_cast<float2*>(smem + p.list_at) + (threadIdx.x - 128);
+        const float over_cap = 1.0f / p.cap;
         int n = 0;                                                 // sums so far
         for (int u = group; u < units && ok; u += groups) {
             const Unit t = unit_of(u);
@@ -668,8 +684,9 @@ __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
             const bool row_on = row < p.n, warp_on = t.x0 + quad * 32 < p.n;
             const int token = row_on ? p.tokens[row] : -1;
             Run mine;
-            float least = row_on && p.k > 0 ? -INFINITY : INFINITY;              // of the list
-            for (int i = 0; i < p.k; ++i) list[i * HEAD_LANES] = make_float2(-INFINITY, __int_as_float(-1));
+            [[maybe_unused]] TopList<TOP> list;
+            [[maybe_unused]] float least = row_on ? -INFINITY : INFINITY;        // of the list
+            if constexpr (TOP > 0) list.clear();
             for (int w0 = t.w0; w0 < t.w_end && ok; w0 += p.bn) {
                 float acc[4][32];                                  // ids 32 half + 64 j and 31 more
                 for (int kb = 0; kb < kb_total; kb += p.part, ++n) {
@@ -722,13 +739,13 @@ __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
 #pragma unroll
                         for (int i = 0; i < 32; ++i) v[i] = c + i < ids ? v[i] : __int_as_float(0x7fffffff);       // no number: nowhere counted
                     }
-                    if (CAP || p.scale != 1.0f) {
+                    if (p.scale != 1.0f) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) v[i] *= p.scale;
                     }
-                    if (CAP) {
+                    if (p.cap > 0.0f) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = p.cap * tanhf(v[i] / p.cap);
+                        for (int i = 0; i < 32; ++i) v[i] = capped(v[i], p.cap, over_cap);
                     }
                     if (token >= first && token < min(first + 32, t.w_end)) {
                         float x = v[0];
@@ -738,24 +755,25 @@ __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
                     }
                     const float most = most_of(v);
                     add_chunk(mine, v, most);
-                    if (__any_sync(0xffffffffu, most > least)) {
-                        uint32_t larger = 0;
+                    if constexpr (TOP > 0) {
+                        if (__any_sync(0xffffffffu, most > least)) {
+                            // every lane puts its next one into its list, until none has any
+                            uint32_t larger = 0;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) larger |= v[i] > least ? 1u << i : 0u;
-                        while (__any_sync(0xffffffffu, larger != 0)) {
-                            const int i = larger ? __ffs(larger) - 1 : 0;
-                            float x[16];
+                            for (int i = 0; i < 32; ++i) larger |= v[i] > least ? 1u << i : 0u;
+                            while (__any_sync(0xffffffffu, larger != 0)) {
+                                const int i = larger ? __ffs(larger) - 1 : 0;
+                                float x[16];
 #pragma unroll
-                            for (int a = 0; a < 16; ++a) x[a] = i & 1 ? v[2 * a + 1] : v[2 * a];
+                                for (int a = 0; a < 16; ++a) x[a] = i & 1 ? v[2 * a + 1] : v[2 * a];
 #pragma unroll
-                            for (int b = 1; b < 5; ++b)
+                                for (int b = 1; b < 5; ++b)
 #pragma unroll
-                                for (int a = 0; a < (16 >> b); ++a) x[a] = (i >> b) & 1 ? x[2 * a + 1] : x[2 * a];
-                            if (larger && x[0] > least) {
-                                list_insert(list, p.k, make_float2(x[0], __int_as_float(first + i)));
-                                least = list[(p.k - 1) * HEAD_LANES].x;
+                                    for (int a = 0; a < (16 >> b); ++a) x[a] = (i >> b) & 1 ? x[2 * a + 1] : x[2 * a];
+                                list.put(larger ? x[0] : -INFINITY, first + i);
+                                larger &= larger - 1;
                             }
-                            larger &= larger - 1;
+                            least = row_on ? list.least(p.k) : INFINITY;
                         }
                     }
                 }
@@ -766,11 +784,10 @@ __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
                 to[0] = mine.m;
                 to[(size_t)parts * p.n] = mine.s;
                 to[(size_t)2 * parts * p.n] = mine.u;
-                u64* keys = p.keys + ((size_t)row * parts + part) * p.k;
-                for (int i = 0; i < p.k; ++i) {
-                    const float2 e = list[i * HEAD_LANES];
-                    const int id = __float_as_int(e.y);
-                    keys[i] = id < 0 ? 0 : key_of(e.x, id);
+                if constexpr (TOP > 0) {
+                    u64* keys = p.keys + ((size_t)row * parts + part) * p.k;
+#pragma unroll
+                    for (int i = 0; i < TOP; ++i) if (i < p.k) keys[i] = list.id[i] < 0 ? 0 : key_of(list.x[i], list.id[i]);
                 }
             }
         }
@@ -849,17 +866,16 @@ static int head_map(CUtensorMap* out, const void* ptr, long long rows, long long
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? AIRUN_OK : AIRUN_ERR_ARG;
 }
 
-template <bool PAIR, bool CAP>
+template <bool PAIR, int TOP>
 static int launch_head(const CUtensorMap& mx, const CUtensorMap& mw, HeadParams p, cudaStream_t stream) {
     static unsigned long long configured = 0;
-    auto kern = head_logprobs_kernel<PAIR, CAP>;
+    auto kern = head_logprobs_kernel<PAIR, TOP>;
     const int w_bytes = p.bn / (PAIR ? 2 : 1) * (BK * 2), x_bytes = p.x_rows * (BK * 2);
     // the products read 128 rows from a stage's first on, in the last one beyond what it brings
-    const int lists = p.k * HEAD_LANES * 8, beyond = 128 * BK * 2 - x_bytes;
-    p.stages = (HEAD_SMEM - 1024 - lists - beyond) / (w_bytes + x_bytes);
+    const int beyond = 128 * BK * 2 - x_bytes;
+    p.stages = (HEAD_SMEM - 1024 - beyond) / (w_bytes + x_bytes);
     if (p.stages > HEAD_STAGES) p.stages = HEAD_STAGES;
-    p.list_at = p.stages * (w_bytes + x_bytes) + beyond;
-    const int smem = 1024 + p.list_at + lists;
+    const int smem = 1024 + p.stages * (w_bytes + x_bytes) + beyond;
     if (first_on_device(configured)) {
         cudaFuncAttributes at;
         cudaError_t e = cudaFuncGetAttributes(&at, kern);
@@ -891,11 +907,11 @@ AIRUN_EXPORT int airun_head_logprobs(const void* x, const void* W, int n, int V,
     const int x_rows = pair || n > 128 ? 128 : (n + 7) / 8 * 8;
     if ((r = head_map(&mx, x, n, K, ldx, x_rows)) != AIRUN_OK) return r;
     if ((r = head_map(&mw, W, V, K, ldw, pair ? bn / 2 : bn)) != AIRUN_OK) return r;
-    HeadParams p = {n, V, K, row_blocks, splits, tiles, bn, part, x_rows, 0, 0, tokens, scale, cap, k, (float*)scratch, nullptr, nullptr, err};
+    HeadParams p = {n, V, K, row_blocks, splits, tiles, bn, part, x_rows, 0, tokens, scale, cap, k, (float*)scratch, nullptr, nullptr, err};
     p.given = p.stats + (size_t)6 * splits * n;
     p.keys = (u64*)((uint8_t*)scratch + ((size_t)4 * (6 * (size_t)splits + 1) * n + 15) / 16 * 16);
-    if (pair) r = cap > 0.0f ? launch_head<true, true>(mx, mw, p, stream) : launch_head<true, false>(mx, mw, p, stream);
-    else r = cap > 0.0f ? launch_head<false, true>(mx, mw, p, stream) : launch_head<false, false>(mx, mw, p, stream);
+    if (pair) r = k == 0 ? launch_head<true, 0>(mx, mw, p, stream) : k <= 8 ? launch_head<true, 8>(mx, mw, p, stream) : launch_head<true, 16>(mx, mw, p, stream);
+    else r = k == 0 ? launch_head<false, 0>(mx, mw, p, stream) : k <= 8 ? launch_head<false, 8>(mx, mw, p, stream) : launch_head<false, 16>(mx, mw, p, stream);
     if (r != AIRUN_OK) return r;
     airun_launch(head_join_kernel, dim3(n), dim3(JOIN_THREADS), 0, stream, (const float*)p.stats, (const float*)p.given, (const u64*)p.keys, tokens, n, V, 2 * splits, k,
                  logprob, entropy, lse, top_ids, top_logprobs);
