@@ -108,11 +108,9 @@ template <int N> __device__ __forceinline__ float most_of(const float (&x)[N]) {
     return most == most ? most : -INFINITY;                        // (all of them not numbers)
 }
 
-__device__ __forceinline__ Part warp_join(Part p) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        p = join(p, Part{__shfl_xor_sync(0xffffffffu, p.m, o), __shfl_xor_sync(0xffffffffu, p.s, o), __shfl_xor_sync(0xffffffffu, p.u, o)});
-    return p;
+__device__ __forceinline__ Part warp_join(const Part& p) {
+    const float m = warp_max(p.m), d = below(p.m, m), f = exp_of(d);
+    return {m, warp_sum(f * p.s), warp_sum(f * fmaf(d, p.s, p.u))};
 }
 
 // The joined part of the block's threads, in its first warp.  `sh` holds one Part a warp.
@@ -158,22 +156,38 @@ template <int NT> struct TopShared {
     u64 group[NT];
     u64 list[CAP];
     u64 top[TOP_MAX];
+    u64 joined[NT >= 256 ? 8 * TOP_MAX : 1];                  // a cluster's lists
     u64 cut;
     int count;
 };
 
-// The k largest of all threads' keys, in order, in sh.top (0 beyond the last).  The threads' keys are all different; `best` is a
-// thread's largest (0: it has none) and each(f) calls f on every key of the thread, or on all that can be as large as `cut`.
+// The k largest of the list's n keys, in order, in sh.top (0 beyond the last): each counts the larger ones.
+template <int NT> __device__ __forceinline__ void rank_top(TopShared<NT>& sh, int n, int k) {
+    const int tid = threadIdx.x;
+    for (int i = tid; i < k; i += NT) if (i >= n) sh.top[i] = 0;
+    for (int i = tid; i < n; i += NT) {
+        const u64 mine = sh.list[i];
+        int larger = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) larger += sh.list[j] > mine || (sh.list[j] == mine && j < i);
+        if (larger < k) sh.top[larger] = mine;
+    }
+    __syncthreads();
+}
+
+// The k largest of all threads' keys, in order, in sh.top; false where more keys than the list holds reach the bound that is found for them.  The
+// threads' keys are all different.  `low` and `high` are bounds of a thread's largest key (0: it has none), the same where it is known, and
+// each(f) calls f on every key of the thread that can be as large as `cut`.
 // The k-th largest of the maxima of groups of threads is a lower bound of the k-th largest of all, and close to it when
 // there are twice as many groups as wanted keys: about k to 2 k keys reach it.  Those are listed and each counts the larger ones.
-// A group is as many lanes as leave 2 k groups; equal logits in every place, whose keys fall with the id, then list
-// k groups' first vectors: 4,096 keys at the most.  A list longer than `few` is cut again in the same way.
-template <int NT, typename Each>
-__device__ __forceinline__ void select_top(TopShared<NT>& sh, u64 best, int k, Each each) {
+// A group is as many lanes as leave 2 k groups, and fewer where logits may come `VEC` neighbours to a thread: equal logits in every place, whose keys
+// fall with the id, list the first vectors of k groups, 512 keys or k NT's least.  A list longer than `few` is cut again in the same way.
+template <int NT, int VEC, typename Each>
+__device__ __forceinline__ bool select_top(TopShared<NT>& sh, u64 low, u64 high, int k, Each each) {
     constexpr int CAP = TopShared<NT>::CAP, MINE = CAP / NT;
     const int tid = threadIdx.x;
     int g = 32;
-    while (g > 1 && NT / g < 2 * k) g >>= 1;
+    while (g > 1 && (NT / g < 2 * k || k * g * VEC > 512)) g >>= 1;
     const int groups = NT / g;
     auto find_cut = [&](u64 b) {
         for (int o = 1; o < g; o <<= 1) {
@@ -198,34 +212,11 @@ __device__ __forceinline__ void select_top(TopShared<NT>& sh, u64 best, int k, E
         const int at = atomicAdd(&sh.count, 1);
         if (at < CAP) sh.list[at] = key;
     };
-    u64 cut = find_cut(best);
-    if (best >= cut) each(cut, [&](u64 key) { if (key >= cut) push(key); });
-    for (int i = tid; i < k; i += NT) sh.top[i] = 0;
+    u64 cut = find_cut(low);
+    if (high >= cut) each(cut, [&](u64 key) { if (key >= cut) push(key); });
     __syncthreads();
     int n = sh.count;
-    if (n > CAP) {
-        // more keys reach the bound than the list holds (large logits that repeat at the threads' stride): one after the other
-        u64 below = ~0ull;
-        for (int i = 0; i < k; ++i) {
-            u64 b = 0;
-            if (best != 0) each(1ull, [&](u64 key) { if (key < below && key > b) b = key; });
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const u64 other = __shfl_xor_sync(0xffffffffu, b, o);
-                b = other > b ? other : b;
-            }
-            __syncthreads();
-            if ((tid & 31) == 0) sh.group[tid >> 5] = b;
-            __syncthreads();
-            b = 0;
-            for (int w = 0; w < NT / 32; ++w) b = sh.group[w] > b ? sh.group[w] : b;
-            if (tid == 0) sh.top[i] = b;
-            below = b;
-            if (b == 0) break;                                   // (the same for all threads)
-        }
-        __syncthreads();
-        return;
-    }
+    if (n > CAP) return false;
     const int few = 2 * k > 128 ? 2 * k : 128;
     for (int round = 0; round < 4 && n > few; ++round) {
         u64 mine[MINE], b = 0;
@@ -242,15 +233,38 @@ __device__ __forceinline__ void select_top(TopShared<NT>& sh, u64 best, int k, E
         if (now >= n) break;
         n = now;
     }
-    for (int i = tid; i < n; i += NT) {
-        const u64 mine = sh.list[i];
-        int larger = 0;
-#pragma unroll 4
-        for (int j = 0; j < n; ++j) larger += sh.list[j] > mine;
-        if (larger < k) sh.top[larger] = mine;
+    rank_top(sh, n, k);
+    return true;
+}
+
+// The same one after the other, for what select_top refuses: large logits that repeat at the threads' stride.
+template <int NT, typename Each>
+__device__ __forceinline__ void one_by_one(TopShared<NT>& sh, int k, Each each) {
+    const int tid = threadIdx.x;
+    u64 below = ~0ull;
+    __syncthreads();
+    for (int i = tid; i < k; i += NT) sh.top[i] = 0;
+    for (int i = 0; i < k; ++i) {
+        u64 b = 0;
+        each(1ull, [&](u64 key) { if (key < below && key > b) b = key; });
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const u64 other = __shfl_xor_sync(0xffffffffu, b, o);
+            b = other > b ? other : b;
+        }
+        __syncthreads();
+        if ((tid & 31) == 0) sh.group[tid >> 5] = b;
+        __syncthreads();
+        b = 0;
+        for (int w = 0; w < NT / 32; ++w) b = sh.group[w] > b ? sh.group[w] : b;
+        if (tid == 0) sh.top[i] = b;
+        below = b;
+        if (b == 0) break;                                       // (the same for all threads)
     }
     __syncthreads();
 }
+// The least logit that reaches a bound.
+__device__ __forceinline__ float cut_logit(u64 cut) { return cut <= 1ull ? -INFINITY : key_logit(cut); }
 
 // ------------------------------------------------------------------ from logits
 struct TokenParams {
@@ -286,17 +300,19 @@ template <> struct Pack<__nv_bfloat16> {
 // A cluster of C blocks a row (C = 1: a block).  The row's 16-byte vectors are dealt to the blocks in turn ranges and, inside, to
 // the threads in batches of U: a thread's elements come by ascending id.  The few elements ahead of the first
 // 16-byte boundary and behind the last belong to the first block's first threads and the last block's first threads.
-template <typename T, int NT, bool CLUSTER>
+// What reaches the bound of the k largest is read again: by few threads, and with C = 1 while the SM's other blocks stream.  TOP: alternatives are wanted.
+template <typename T, int NT, bool CLUSTER, bool TOP>
 __global__ __launch_bounds__(NT) void token_logprobs_kernel(const TokenParams p, int n_parts) {
     pdl_trigger();
     constexpr int VEC = Pack<T>::N, U = 4;
     __shared__ TopShared<NT> top;
     __shared__ Part s_parts[32];
-    __shared__ Part s_mine;
+    __shared__ Part s_part_of[8];                                // of the cluster's blocks, in the first one's memory
     __shared__ Row s_row;
     const int tid = threadIdx.x;
     const int part = CLUSTER ? (int)cluster_rank() : 0, parts = CLUSTER ? n_parts : 1;
     const int r = CLUSTER ? blockIdx.x / parts : blockIdx.x;
+    if (CLUSTER) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     pdl_wait();
     const int at = p.rows ? p.rows[r] : r;
     const int token = p.tokens[r];
@@ -308,31 +324,31 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(const TokenParams p,
 
     const int lead = min(V, (int)((16 - ((uintptr_t)row & 15)) % 16 / sizeof(T)));
     const int vecs = (V - lead) / VEC, tail = lead + vecs * VEC;
-    const int v0 = (int)((long long)vecs * part / parts), v1 = (int)((long long)vecs * (part + 1) / parts);
-    const int n_batches = (v1 - v0 + U * NT - 1) / (U * NT);
+    const int v0 = (int)((long long)vecs * part / parts) + tid, v1 = (int)((long long)vecs * (part + 1) / parts);      // this thread's first; the block's end
+    const int n_batches = v0 < v1 ? (v1 - v0 + U * NT - 1) / (U * NT) : 0;
     const Pack<T>* from = reinterpret_cast<const Pack<T>*>(row + lead);
     // the element ahead of the vectors that is this thread's, and the one behind them
     const int ahead = part == 0 && tid < lead ? tid : -1, behind = part == parts - 1 && tid < V - tail ? tail + tid : -1;
 
     Run mine;
-    float second = -INFINITY;                                    // largest of the batches but the one with the maximum
-    int best_batch = -1;
-    if (ahead >= 0) {
-        const float x[2] = {to_f32<T>(row[ahead]), -INFINITY};
-        add_chunk(mine, x, most_of(x));
-        second = mine.m;                                         // (its own key is looked at below)
-    }
-    for (int b = 0; b < n_batches; ++b) {
+    float x[U * VEC];                                            // a batch; what is not a number becomes minus infinity
+    auto load = [&](int b) {
         Pack<T> in[U];
-        const int first = v0 + b * U * NT + tid;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            if (first + i * NT < v1) in[i] = from[first + i * NT];
+            const int v = v0 + (b * U + i) * NT;
+            if (v < v1) in[i] = from[v];
             else in[i].nothing();
         }
-        float x[U * VEC];
 #pragma unroll
         for (int i = 0; i < U * VEC; ++i) x[i] = in[i / VEC].at(i % VEC);
+    };
+    auto id_of = [&](int b, int i) { return lead + (v0 + (b * U + i / VEC) * NT) * VEC + i % VEC; };
+    float second = -INFINITY;                                    // largest of the batches but the one with the maximum
+    int best_batch = -1;
+    const float one_ahead = ahead >= 0 ? to_f32<T>(row[ahead]) : -INFINITY, one_behind = behind >= 0 ? to_f32<T>(row[behind]) : -INFINITY;
+    for (int b = 0; b < n_batches; ++b) {
+        load(b);
         const float most = most_of(x);
         if (most > mine.m) {
             if (best_batch >= 0) second = mine.m;
@@ -342,79 +358,74 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(const TokenParams p,
         }
         add_chunk(mine, x, most);
     }
-    if (behind >= 0) {
-        const float x[2] = {to_f32<T>(row[behind]), -INFINITY};
-        add_chunk(mine, x, most_of(x));
+    const float most = mine.m;                                   // of the vectors
+    if (ahead >= 0 || behind >= 0) {
+        const float ends[2] = {one_ahead, one_behind};
+        add_chunk(mine, ends, most_of(ends));
     }
 
-    if (p.k > 0) {
-        auto vectors = [&](int b, auto f) {
-            const int first = v0 + b * U * NT + tid;
+    if constexpr (TOP) {
+        u64 end_best = 0;
+        if (ahead >= 0) end_best = key_of(one_ahead, ahead);
+        if (behind >= 0) end_best = max(end_best, key_of(one_behind, behind));
+        auto ends = [&](auto f) {
+            if (ahead >= 0) f(key_of(one_ahead, ahead));
+            if (behind >= 0) f(key_of(one_behind, behind));
+        };
+        // the keys of the batch in x that can reach the bound
+        auto batch = [&](int b, u64 cut, auto f) {
+            const float least = cut_logit(cut);
 #pragma unroll
-            for (int i = 0; i < U; ++i) {
-                if (first + i * NT >= v1) break;
-                const Pack<T> x = from[first + i * NT];
-                const int id = lead + (first + i * NT) * VEC;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) f(key_of(x.at(j), id + j));
+            for (int i = 0; i < U * VEC; ++i)
+                if (!(x[i] < least) && v0 + (b * U + i / VEC) * NT < v1) f(key_of(x[i], id_of(b, i)));
+        };
+        auto each = [&](u64 cut, auto f) {
+            ends(f);
+            if (best_batch >= 0 && key_of(second, 0) < cut) {    // no other batch reaches the bound
+                load(best_batch);
+                batch(best_batch, cut, f);
+                return;
+            }
+            for (int b = 0; b < n_batches; ++b) {
+                if (best_batch < 0 && key_of(-INFINITY, id_of(b, 0)) < cut) break;        // (equal ones go on falling with their ids)
+                load(b);
+                batch(b, cut, f);
             }
         };
-        auto every = [&](auto f) {
-            if (ahead >= 0) f(key_of(to_f32<T>(row[ahead]), ahead));
-            for (int b = 0; b < n_batches; ++b) vectors(b, f);
-            if (behind >= 0) f(key_of(to_f32<T>(row[behind]), behind));
-        };
-        u64 best = 0;
-        auto raise = [&](u64 key) { best = key > best ? key : best; };
-        if (ahead >= 0) raise(key_of(to_f32<T>(row[ahead]), ahead));
-        if (behind >= 0) raise(key_of(to_f32<T>(row[behind]), behind));
-        if (best_batch >= 0) vectors(best_batch, raise);
-        else if (n_batches > 0) vectors(0, raise);               // nothing but minus infinity: the first ids
-        select_top<NT>(top, best, p.k, [&](u64 cut, auto f) {
-            const bool one = best_batch >= 0 && key_of(second, 0) < cut;       // no other batch reaches the bound
-            if (!one) { every(f); return; }
-            if (ahead >= 0) f(key_of(to_f32<T>(row[ahead]), ahead));
-            vectors(best_batch, f);
-            if (behind >= 0) f(key_of(to_f32<T>(row[behind]), behind));
-        });
+        // The largest of the vectors lies somewhere in its batch: from the first to the last id of it, unless there is nothing but minus infinity.
+        u64 low = end_best, high = end_best;
+        if (n_batches > 0) {
+            const int b = max(best_batch, 0);
+            high = max(high, key_of(most, id_of(b, 0)));
+            low = max(low, key_of(most, best_batch < 0 ? id_of(b, 0) : id_of(b, U * VEC - 1)));
+        }
+        if (!select_top<NT, VEC>(top, low, high, p.k, each)) {
+            // many equal ones: with the places of the maxima, the first ids are told from the others
+            u64 best = end_best;
+            if (n_batches > 0) {
+                load(max(best_batch, 0));
+                batch(max(best_batch, 0), key_of(most, 0x7fffffff), [&](u64 key) { best = max(best, key); });
+            }
+            if (!select_top<NT, VEC>(top, best, best, p.k, each)) one_by_one<NT>(top, p.k, each);
+        }
     }
     Part all = block_join<NT>(mine.part(), s_parts);
     if (CLUSTER) {
-        if (tid == 0) s_mine = all;
-        cluster_sync_all();
-        if (part == 0) {
-            if (tid < 32) {
-                Part q = {-INFINITY, 0.0f, 0.0f};
-                if (tid < parts) {
-                    const uint32_t a = map_to_cta((uint32_t)__cvta_generic_to_shared(&s_mine), (uint32_t)tid);
-                    q = {ld_cluster_f32(a), ld_cluster_f32(a + 4), ld_cluster_f32(a + 8)};
-                }
-                all = warp_join(q);
-            }
-            if (p.k > 0) {
-                const uint32_t tops = (uint32_t)__cvta_generic_to_shared(top.top);
-                auto key_at = [&](int i) {
-                    u64 key;
-                    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key) : "r"(map_to_cta(tops, (uint32_t)(i / p.k)) + 8u * (uint32_t)(i % p.k)) : "memory");
-                    return key;
-                };
-                // (at most 8 blocks of 128 keys; this block's own list is overwritten, so all are read first)
-                constexpr int MOST = (8 * TOP_MAX + NT - 1) / NT;
-                u64 mine_k[MOST], best = 0;
-#pragma unroll
-                for (int i = 0; i < MOST; ++i) {
-                    const int j = tid + i * NT;
-                    mine_k[i] = j < parts * p.k ? key_at(j) : 0;
-                    best = mine_k[i] > best ? mine_k[i] : best;
-                }
-                select_top<NT>(top, best, p.k, [&](u64, auto f) {
-#pragma unroll
-                    for (int i = 0; i < MOST; ++i) if (mine_k[i]) f(mine_k[i]);
-                });
-            }
+        // every block stores its part and its list into the first one's memory, and all but that one may leave
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");         // every block runs: its memory may be written
+        if (tid == 0) {
+            const uint32_t to = map_to_cta((uint32_t)__cvta_generic_to_shared(&s_part_of[part]), 0);
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(all.m) : "memory");
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(all.s) : "memory");
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(all.u) : "memory");
         }
-        cluster_sync_all();                                      // nobody leaves while its memory is read
+        if constexpr (TOP) {
+            const uint32_t to = map_to_cta((uint32_t)__cvta_generic_to_shared(top.joined) + 8u * (uint32_t)(part * p.k), 0);
+            for (int i = tid; i < p.k; i += NT) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to + 8u * (uint32_t)i), "l"(top.top[i]) : "memory");
+        }
+        cluster_sync_all();
         if (part != 0) return;
+        if (tid < 32) all = warp_join(tid < parts ? s_part_of[tid] : Part{-INFINITY, 0.0f, 0.0f});
     }
     if (tid == 0) {
         const Row w = row_of(all);
@@ -423,9 +434,21 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(const TokenParams p,
         if (p.lse) p.lse[r] = row_lse(w);
         if (p.entropy) p.entropy[r] = w.entropy;
     }
-    if (p.k > 0) {
+    if constexpr (TOP) {
         __syncthreads();
         const Row w = s_row;
+        if (CLUSTER) {
+            // 8 lists of 128 at the most: each key counts the larger ones
+            const int n_keys = parts * p.k;
+            for (int i = tid; i < n_keys; i += NT) {
+                const u64 mine_k = top.joined[i];
+                int larger = 0;
+#pragma unroll 8
+                for (int j = 0; j < n_keys; ++j) larger += top.joined[j] > mine_k || (top.joined[j] == mine_k && j < i);
+                if (larger < p.k) top.top[larger] = mine_k;
+            }
+            __syncthreads();
+        }
         for (int i = tid; i < p.k; i += NT) {
             const u64 key = top.top[i];
             p.top_ids[(size_t)r * p.k + i] = key ? key_id(key) : -1;
@@ -434,16 +457,26 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(const TokenParams p,
     }
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool TOP>
 static int launch_tokens(const TokenParams& p, int n, int parts, cudaStream_t stream) {
     if constexpr (NT == 512) {
         if (parts > 1) {
-            airun_launch_clusters(token_logprobs_kernel<T, NT, true>, dim3(n * parts), dim3(NT), 0, stream, dim3(parts), p, parts);
+            airun_launch_clusters(token_logprobs_kernel<T, NT, true, TOP>, dim3(n * parts), dim3(NT), 0, stream, dim3(parts), p, parts);
             return airun_launch_status();
         }
     }
-    airun_launch(token_logprobs_kernel<T, NT, false>, dim3(n), dim3(NT), 0, stream, p, 1);
+    airun_launch(token_logprobs_kernel<T, NT, false, TOP>, dim3(n), dim3(NT), 0, stream, p, 1);
     return airun_launch_status();
+}
+
+template <typename T>
+static int launch_tokens(const TokenParams& p, int n, cudaStream_t stream) {
+    if (p.V <= 2048) return p.k > 0 ? launch_tokens<T, 128, true>(p, n, 1, stream) : launch_tokens<T, 128, false>(p, n, 1, stream);
+    // a block a row once there are rows for the SMs; below, rows in up to 8 parts of 4,096 logits and more
+    const int sms = airun_sm_count();
+    int parts = 1;
+    while (parts < 8 && 2 * parts * n <= 2 * sms && p.V / (2 * parts) >= 4096) parts *= 2;
+    return p.k > 0 ? launch_tokens<T, 512, true>(p, n, parts, stream) : launch_tokens<T, 512, false>(p, n, parts, stream);
 }
 
 // logits: [held][V] rows ld elements apart; rows: [n] or null (then held >= n); tokens, logprob, entropy, lse: [n]; top_*: [n][k].
@@ -454,12 +487,8 @@ AIRUN_EXPORT int airun_token_logprobs(const void* logits, int dtype, long long l
     if (n == 0) return AIRUN_OK;
     if (!logits || !tokens || !logprob || (k > 0 && (!top_ids || !top_logprobs)) || (!rows && n > held)) return AIRUN_ERR_ARG;
     const TokenParams p = {logits, ld, held, V, rows, tokens, logprob, entropy, lse, k, top_ids, top_logprobs, err};
-    const int sms = airun_sm_count();
-    // a block a row once there are rows for the SMs; below, rows in up to 8 parts of 4,096 logits and more
-    int parts = 1;
-    while (parts < 8 && 2 * parts * n <= 2 * sms && V / (2 * parts) >= 4096) parts *= 2;
-    if (dtype == AIRUN_DT_F32) return V <= 2048 ? launch_tokens<float, 128>(p, n, 1, stream) : launch_tokens<float, 512>(p, n, parts, stream);
-    if (dtype == AIRUN_DT_BF16) return V <= 2048 ? launch_tokens<__nv_bfloat16, 128>(p, n, 1, stream) : launch_tokens<__nv_bfloat16, 512>(p, n, parts, stream);
+    if (dtype == AIRUN_DT_F32) return launch_tokens<float>(p, n, stream);
+    if (dtype == AIRUN_DT_BF16) return launch_tokens<__nv_bfloat16>(p, n, stream);
     return AIRUN_ERR_UNSUPPORTED;
 }
 
@@ -824,9 +853,10 @@ __global__ __launch_bounds__(JOIN_THREADS) void head_join_kernel(
         const u64* mine_k = keys + (size_t)r * parts * k;
         u64 best = 0;
         for (int i = tid; i < parts * k; i += JOIN_THREADS) best = mine_k[i] > best ? mine_k[i] : best;
-        select_top<JOIN_THREADS>(top, best, k, [&](u64, auto f) {
+        auto each = [&](u64, auto f) {
             for (int i = tid; i < parts * k; i += JOIN_THREADS) if (mine_k[i]) f(mine_k[i]);
-        });
+        };
+        if (!select_top<JOIN_THREADS, 1>(top, best, best, k, each)) one_by_one<JOIN_THREADS>(top, k, each);
         if (tid == 0) {
             int at = 0, id = 0;
             while (at < k && top.top[at]) ++at;

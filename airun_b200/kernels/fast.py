@@ -46,6 +46,9 @@ _MACHINES: Dict[object, Machine] = {}
 
 def machine(device=None) -> Machine:
     """The Machine of ``device`` (default: the current CUDA device; without a GPU, a B200's numbers)."""
+    known = getattr(device, "index", None)
+    if isinstance(known, int) and known in _MACHINES:      # a GPU seen before (asking whether there is one takes 4 us)
+        return _MACHINES[known]
     if not torch.cuda.is_available():
         return _MACHINES.setdefault(None, Machine(B200_SMS))
     idx = torch.device(device).index if device is not None and torch.device(device).index is not None \
@@ -427,13 +430,16 @@ def head_logprobs_bf16(hidden, weight, tokens, logprob, entropy, lse, top_ids, t
         return False
     pair, splits, tiles, bn, part = plan_head(n, V, K, machine(hidden.device).sms)
     scratch = alloc(((4 * (6 * splits + 1) * n + 15) // 16 * 16 + 16 * splits * n * k,), torch.uint8)
-    f = _fn("logprobs", "airun_head_logprobs",
-            [c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_void_p, c_float, c_float, c_int, c_int, c_int, c_int, c_int, c_void_p,
-             c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p])
-    _check(f(_p(hidden), _p(weight), n, V, K, hidden.stride(0) if n > 1 else max(K, hidden.stride(0)), weight.stride(0) if V > 1 else max(K, weight.stride(0)),
-             _p(tokens), float(scale), float(soft_cap or 0.0), 1 if pair else 0, splits, tiles, bn, part, _p(scratch), _p(logprob), _p(entropy), _p(lse), k,
-             _p(top_ids), _p(top_logprobs), _p(err), _stream()), "head_logprobs")
+    f = _fn("logprobs", "airun_head_logprobs", _HEAD_LOGPROBS)
+    at = ops._at
+    _check(f(hidden.data_ptr(), weight.data_ptr(), n, V, K, hidden.stride(0) if n > 1 else max(K, hidden.stride(0)),
+             weight.stride(0) if V > 1 else max(K, weight.stride(0)), tokens.data_ptr(), scale, soft_cap or 0.0, 1 if pair else 0, splits, tiles, bn, part,
+             scratch.data_ptr(), logprob.data_ptr(), at(entropy), at(lse), k, at(top_ids), at(top_logprobs), err.data_ptr(), _stream()), "head_logprobs")
     return True
+
+
+_HEAD_LOGPROBS = [c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_void_p, c_float, c_float, c_int, c_int, c_int, c_int, c_int, c_void_p,
+                  c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p]
 
 
 def linear_swiglu_bf16(ctx, x: torch.Tensor, w_gu: torch.Tensor, out: torch.Tensor, group: int, normed=None) -> bool:

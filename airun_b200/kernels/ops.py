@@ -42,7 +42,12 @@ def _p(t: Optional[torch.Tensor]):
     return None if t is None else c_void_p(t.data_ptr())
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)     # of a device; current_stream() makes an object of it, 4 us
+
+
 def _stream() -> c_void_p:
+    if _raw_stream is not None:
+        return c_void_p(_raw_stream(torch.cuda.current_device()))
     return c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
@@ -57,11 +62,17 @@ def _cuda(*ts: Optional[torch.Tensor]) -> None:
             _need(t.is_cuda, "kernel arguments must live on the GPU (there is no CPU path)")
 
 
-def _one_device(*ts: Optional[torch.Tensor]) -> None:
+def _here(*ts: Optional[torch.Tensor]) -> None:
     """All on the current device, whose stream the kernel is launched on."""
     here = torch.cuda.current_device()
     for t in ts:
-        _need(t is None or t.device.index == here, "kernel arguments must live on the current device")
+        if t is not None and t.get_device() != here:
+            _cuda(t)
+            raise KernelError("kernel arguments must live on the current device")
+
+
+def _at(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 LAUNCHES = [0]          # kernels launched through this module (CUDA-graph replays are counted by their owner)
@@ -82,7 +93,7 @@ _SIGS = {}
 
 
 def _fn(lib_name: str, fn_name: str, argtypes, defines=None):
-    key = (lib_name, fn_name, tuple(sorted((defines or {}).items())))
+    key = (lib_name, fn_name, tuple(sorted(defines.items())) if defines else ())
     f = _SIGS.get(key)
     if f is None:
         lib = build.load(lib_name, defines)
@@ -1270,23 +1281,24 @@ def largest_logits(logits: torch.Tensor, rows: torch.Tensor, n: int, n_cand: int
 TOP_LOGPROBS_MAX = 128
 
 
-def _logprob_outputs(tokens: torch.Tensor, vocab: int, logprob, entropy, lse, top_ids, top_logprobs) -> int:
+def _logprob_outputs(n: int, vocab: int, tokens, logprob, entropy, lse, top_ids, top_logprobs) -> int:
     """Checks the given tokens and the places for their results; returns how many alternatives are asked for."""
-    _cuda(tokens, logprob, entropy, lse, top_ids, top_logprobs)
-    _need(tokens.dtype == torch.int32 and tokens.dim() == 1 and tokens.is_contiguous(), "tokens must be int32 [n]")
-    n = tokens.shape[0]
+    if tokens.dtype != torch.int32 or tokens.dim() != 1 or not tokens.is_contiguous():
+        raise KernelError("tokens must be int32 [n]")
+    size = (n,)
     for t in (logprob, entropy, lse):
-        _need(t is None or (t.dtype == torch.float32 and tuple(t.shape) == (n,) and t.is_contiguous()),
-              "logprob, entropy and lse must be float32 [n]")
-    _need((top_ids is None) == (top_logprobs is None), "the alternatives' ids and log probabilities come together")
-    if top_ids is None:
+        if t is not None and (t.dtype != torch.float32 or t.shape != size or not t.is_contiguous()):
+            raise KernelError("logprob, entropy and lse must be float32 [n]")
+    if top_ids is None or top_logprobs is None:
+        _need(top_ids is top_logprobs, "the alternatives' ids and log probabilities come together")
         return 0
-    _need(top_ids.dim() == 2 and top_ids.shape[0] == n and 1 <= top_ids.shape[1] <= min(TOP_LOGPROBS_MAX, vocab),
-          f"the alternatives are [n, k] with k from 1 to {TOP_LOGPROBS_MAX} and to the vocabulary")
-    _need(top_ids.dtype == torch.int32 and top_ids.is_contiguous() and top_logprobs.dtype == torch.float32
-          and top_logprobs.shape == top_ids.shape and top_logprobs.is_contiguous(),
-          "the alternatives' ids must be int32 and their log probabilities float32, contiguous and of one shape")
-    return top_ids.shape[1]
+    shape = top_ids.shape
+    if len(shape) != 2 or shape[0] != n or not 1 <= shape[1] <= min(TOP_LOGPROBS_MAX, vocab):
+        raise KernelError(f"the alternatives are [n, k] with k from 1 to {TOP_LOGPROBS_MAX} and to the vocabulary")
+    if (top_ids.dtype != torch.int32 or not top_ids.is_contiguous() or top_logprobs.dtype != torch.float32 or top_logprobs.shape != shape
+            or not top_logprobs.is_contiguous()):
+        raise KernelError("the alternatives' ids must be int32 and their log probabilities float32, contiguous and of one shape")
+    return shape[1]
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tensor, entropy: Optional[torch.Tensor] = None,
@@ -1304,21 +1316,25 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Te
     entropy 0, one with plus infinity the entropy NaN; a token outside [0, V) has minus infinity, so rows that are padding may ask for
     -1.  A row index outside [0, R) reads nothing: it gives what a row without a distribution does, with ids of -1, and sets
     the bit of a bad row in ``err``, if that is given."""
-    _cuda(logits, rows, err)
-    _need(logits.dim() == 2 and logits.shape[1] > 0 and logits.stride(1) == 1, "logits must be row-major [rows, V]")
-    R, V = logits.shape
-    k = _logprob_outputs(tokens, V, logprob, entropy, lse, top_ids, top_logprobs)
-    n = tokens.shape[0]
-    _need(rows is None or (rows.dtype == torch.int32 and tuple(rows.shape) == (n,) and rows.is_contiguous()), "rows must be int32 [n]")
-    _need(rows is not None or R >= n, "a row of logits for every token")
-    _need(R <= 1 or logits.stride(0) >= V, "rows of logits must not overlap")
-    _one_device(logits, tokens, logprob, entropy, lse, top_ids, top_logprobs, rows, err)
-    f = _fn("logprobs", "airun_token_logprobs", [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
-                                                 c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p])
-    _check(f(_p(logits), _dt(logits), logits.stride(0) if R > 1 else V, R, V, _p(rows), _p(tokens), n, _p(logprob), _p(entropy), _p(lse), k,
-             _p(top_ids), _p(top_logprobs), _p(err), _stream()), "token_logprobs")
+    _here(logits, tokens, logprob, entropy, lse, top_ids, top_logprobs, rows, err)
+    shape, n = logits.shape, tokens.shape[0]
+    if len(shape) != 2 or shape[1] == 0 or logits.stride(1) != 1:
+        raise KernelError("logits must be row-major [rows, V]")
+    R, V = shape
+    k = _logprob_outputs(n, V, tokens, logprob, entropy, lse, top_ids, top_logprobs)
+    if rows is None:
+        _need(R >= n, "a row of logits for every token")
+    else:
+        _need(rows.dtype == torch.int32 and rows.shape == (n,) and rows.is_contiguous() and (R > 0 or n == 0), "rows must be int32 [n], of one row of logits or more")
+    ld = logits.stride(0) if R > 1 else V
+    _need(ld >= V, "rows of logits must not overlap")
+    f = _fn("logprobs", "airun_token_logprobs", _TOKEN_LOGPROBS)
+    _check(f(logits.data_ptr(), _dt(logits), ld, R, V, _at(rows), tokens.data_ptr(), n, logprob.data_ptr(), _at(entropy), _at(lse), k, _at(top_ids),
+             _at(top_logprobs), _at(err), _stream()), "token_logprobs")
 
 
+_TOKEN_LOGPROBS = [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                   c_void_p, c_void_p]
 _cap = soft_cap                        # (an argument has the name below)
 HEAD_CHUNK = 1 << 26                   # logits that are held at a time where they are formed at all: 256 MiB
 
@@ -1332,19 +1348,19 @@ def head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tens
     ``ws``: an engine.batch.Workspace to take scratch from (None: allocated).  Scratch is in use until the call's kernels are done:
     calls that may overlap on the GPU (two streams, two graphs) need workspaces of their own.  ``err``: int32 [1], the device-side
     error word."""
-    _cuda(hidden, weight, err)
-    _need(hidden.dim() == 2 and weight.dim() == 2 and hidden.shape[1] == weight.shape[1] and weight.shape[0] > 0 and weight.shape[1] > 0,
-          "hidden [n, H] and weight [V, H] do not agree")
+    _here(hidden, weight, tokens, logprob, err, entropy, lse, top_ids, top_logprobs)
+    hs, wsh = hidden.shape, weight.shape
+    if len(hs) != 2 or len(wsh) != 2 or hs[1] != wsh[1] or wsh[0] == 0 or wsh[1] == 0:
+        raise KernelError("hidden [n, H] and weight [V, H] do not agree")
     _need(hidden.dtype == weight.dtype, "hidden and weight must share a type")
-    _need(hidden.stride(1) == 1 and weight.stride(1) == 1, "hidden and weight must be row-major")
-    n, V = hidden.shape[0], weight.shape[0]
-    _need(tokens.dim() == 1 and tokens.shape[0] == n, "a token for every row")
-    k = _logprob_outputs(tokens, V, logprob, entropy, lse, top_ids, top_logprobs)
-    _need(err.dtype == torch.int32 and err.numel() == 1, "err must be one int32")
-    _need(scale == scale and abs(scale) < float("inf"), "the scale must be finite")
-    _need(soft_cap is None or 0.0 < soft_cap < float("inf"), "the cap must be positive")
     _dt(hidden)
-    _one_device(hidden, weight, tokens, logprob, entropy, lse, top_ids, top_logprobs, err)
+    _need(hidden.stride(1) == 1 and weight.stride(1) == 1, "hidden and weight must be row-major")
+    n, V = hs[0], wsh[0]
+    _need(tokens.dim() == 1 and tokens.shape[0] == n, "a token for every row")
+    _logprob_outputs(n, V, tokens, logprob, entropy, lse, top_ids, top_logprobs)
+    _need(err.dtype == torch.int32 and err.numel() == 1, "err must be one int32")
+    _need(abs(scale) < float("inf"), "the scale must be finite")
+    _need(soft_cap is None or 0.0 < soft_cap < float("inf"), "the cap must be positive")
     if n == 0:
         return
     alloc = ws.alloc if ws is not None else (lambda shape, dtype: torch.empty(shape, dtype=dtype, device=hidden.device))

@@ -362,7 +362,7 @@ class _Fake:
 def test_refusals(monkeypatch):
     from airun_b200.kernels import ops
     monkeypatch.setattr(ops, "_fn", lambda *a, **k: pytest.fail("launched"))
-    monkeypatch.setattr(ops, "_one_device", lambda *a: None)
+    monkeypatch.setattr(ops, "_here", ops._cuda)
     x, t, lp = _Fake(4, 100), _Fake(4, dtype=torch.int32), _Fake(4)
 
     def refused(match, logits=x, tokens=t, logprob=lp, **kw):
@@ -381,6 +381,7 @@ def test_refusals(monkeypatch):
     refused("to the vocabulary", logits=_Fake(4, 999), top_ids=_Fake(4, 129, dtype=torch.int32), top_logprobs=_Fake(4, 129))
     refused("one shape", top_ids=_Fake(4, 3, dtype=torch.int32), top_logprobs=_Fake(4, 2))
     refused("int32", rows=_Fake(5, dtype=torch.int32))
+    refused("one row", rows=t, logits=_Fake(0, 100))
     monkeypatch.setattr(ops, "_fn", lambda *a, **k: (lambda *b: 0))
     refused("dtype", logits=_Fake(4, 100, dtype=torch.float16))
 
@@ -388,7 +389,7 @@ def test_refusals(monkeypatch):
 def test_head_refusals(monkeypatch):
     from airun_b200.kernels import ops
     monkeypatch.setattr(ops, "_fn", lambda *a, **k: pytest.fail("launched"))
-    monkeypatch.setattr(ops, "_one_device", lambda *a: None)
+    monkeypatch.setattr(ops, "_here", ops._cuda)
     h, w, t, lp, err = _Fake(4, 64), _Fake(100, 64), _Fake(4, dtype=torch.int32), _Fake(4), _Fake(1, dtype=torch.int32)
 
     def refused(match, hidden=h, weight=w, tokens=t, logprob=lp, err=err, **kw):
