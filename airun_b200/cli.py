@@ -274,6 +274,8 @@ def cmd_perplexity(a) -> int:
     import math
     import torch
     from . import Engine, EngineOptions, StepEntry
+    from .kernels import ops
+    from .parts.base import TokenScores
     if not a.file:
         raise SystemExit("perplexity needs --file with the token ids to score (the engine has no tokenizer)")
     with open(a.file) as f:
@@ -298,29 +300,34 @@ def cmd_perplexity(a) -> int:
     losses = []                                    # (position, token, loss)
     total, top1 = 0.0, 0
 
-    def score(logits_row, pos):
+    def note(scores, first):
+        """Scores of the tokens at the places from ``first`` on; their log probabilities are worked out on the GPU."""
         nonlocal total, top1
-        logp = torch.log_softmax(logits_row.double(), dim=-1)
-        nll = -float(logp[ids[pos]])
-        top1 += int(int(torch.argmax(logits_row)) == ids[pos])
-        total += nll
-        losses.append((pos, ids[pos], nll))
+        for k, (lp, best) in enumerate(zip(scores.logprob.tolist(), scores.top_ids[:, 0].tolist())):
+            pos = first + k
+            top1 += int(best == ids[pos])
+            total -= lp
+            losses.append((pos, ids[pos], -lp))
+
+    one = TokenScores.empty(1, 1, eng.device)
+    target = torch.zeros(1, dtype=torch.int32, device=eng.device)
 
     for start, end, first in passes:
         slot = eng.manager.add_request("t").slot   # an empty context for every pass
         eng.storage.zero_state_slot(slot)
         if a.batched:
             rows = [r for r in range(end - start) if r >= first and r + 1 < end - start]
-            logits = eng.runner.step([StepEntry("t", ids[start:end], tuple(rows))])
-            host = logits.float().cpu() if logits is not None else None
-            for k, r in enumerate(rows):
-                score(host[k], start + r + 1)
+            scores = eng.runner.score([StepEntry("t", ids[start:end], tuple(rows))], [ids[start + r + 1] for r in rows], top=1)
+            if scores is not None:
+                note(scores, start + rows[0] + 1)
         else:
             for i in range(start, end - 1):
                 wanted = i - start >= first
                 logits = eng.runner.step([StepEntry("t", [ids[i]], (0,) if wanted else ())])
                 if wanted:
-                    score(logits.float().cpu()[0], i + 1)
+                    target.fill_(ids[i + 1])
+                    ops.token_logprobs(logits, target, one.logprob, one.entropy, None, one.top_ids, one.top_logprobs)
+                    note(one, i + 1)
         eng.manager.free_request("t")
         if len(passes) > 1:
             print(f"[{len(losses) // max(end - start - 1 - first, 1)}]{math.exp(total / max(len(losses), 1)):.4f},",

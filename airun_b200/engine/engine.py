@@ -15,15 +15,15 @@ import itertools
 import os
 import time
 from dataclasses import dataclass
-from typing import Hashable, List, Optional, Sequence, Union
+from typing import Dict, Hashable, List, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
 
-from ..cache.manager import CacheManager, CacheStorage
+from ..cache.manager import CacheManager, CacheStorage, OutOfPages, OutOfSlots
 from ..config.base import ModelConfig, architecture_name, load_config, lookup_architecture, read_config_json
 from ..kernels import ops
-from ..sampling.sampler import SamplingParams, sample_candidates, sample_rows
+from ..sampling.sampler import SamplingParams, TokenProbs, sample_candidates, sample_rows
 from ..weights.loader import open_model_folder
 from .scheduler import FinishReason, Request, Scheduler
 from .step import StepEntry, StepRunner
@@ -78,6 +78,21 @@ class GenerationResult:
     logprobs: Optional[list] = None          # TokenProbs per sampled token when SamplingParams.logprobs is set
 
 
+@dataclass
+class PromptScore:
+    """A prompt's tokens under the model: ``logprobs[i]`` and ``entropies[i]`` (nats) are those of token i given the ones before it, ``top[i]`` the
+    likeliest tokens there with their log probabilities, the best first; the first token has none (None, and an empty list)."""
+    token_ids: List[int]
+    logprobs: List[Optional[float]]
+    entropies: List[Optional[float]]
+    top: List[List[Tuple[int, float]]]
+
+    @property
+    def total(self) -> float:
+        """ln of the probability of all tokens behind the first."""
+        return float(sum(self.logprobs[1:]))
+
+
 class Engine:
     def __init__(self, config: ModelConfig, model, options: EngineOptions):
         self.config, self.model, self.options = config, model, options
@@ -110,6 +125,7 @@ class Engine:
         self.stats = GenerationStats()
         self._ahead = None        # (requests, prepared step): the next decode step, laid out while this one runs
         self._host_rows = None    # buffers for the logits rows the host samples
+        self._prob_bufs = None    # buffers for the log probabilities of the tokens picked
         self._cand_bufs = None    # buffers for the largest logits of the rows whose chain cuts to them anyway
         # AIRUN_NARROW_ROWS=0: every row the host samples travels whole (the plain way; tests compare the two)
         self._narrow_rows = os.environ.get("AIRUN_NARROW_ROWS", "1") != "0"
@@ -314,7 +330,7 @@ class Engine:
         host = self._small_host.numpy()
         for i, r in enumerate(reqs):
             p = r.params
-            dev = r.sampler.device_ok
+            dev = self._drawer(r).device_ok
             host[i] = p.temperature if (dev and p.temperature > 0.0) else 0.0
             host[R + i] = r.sampler.next_uniform() if (dev and p.temperature > 0.0) else 0.0
         self._small_dev.copy_(self._small_host, non_blocking=True)
@@ -325,9 +341,10 @@ class Engine:
         # their largest logits to the host (found on the device), the others their whole row.
         cand_rows, host_rows, n_cand = [], [], 0
         for i, r in enumerate(reqs):
-            if r.sampler.device_ok:
+            drawer = self._drawer(r)
+            if drawer.device_ok:
                 continue
-            need = r.sampler.candidates_needed if self._narrow_rows else 0
+            need = drawer.candidates_needed if self._narrow_rows else 0
             if need > 0:
                 cand_rows.append(i)
                 n_cand = max(n_cand, need)
@@ -335,6 +352,8 @@ class Engine:
                 host_rows.append(i)
         cands = self._candidates_to_host(logits, cand_rows, n_cand) if cand_rows else None
         rows_host = self._rows_to_host(logits, host_rows) if host_rows else None
+        prob_rows = [i for i, r in enumerate(reqs) if r.params.logprobs is not None and i not in set(host_rows)]
+        probs = self._probs_to_host(logits, prob_rows, max(reqs[i].params.logprobs for i in prob_rows)) if prob_rows else None
         if look_ahead and not host_rows and self._ahead is None:
             self._prepare_ahead(reqs)                      # the GPU is busy: plan and lay out the next step meanwhile
         torch.cuda.current_stream().synchronize()
@@ -344,6 +363,10 @@ class Engine:
             self.runner.err.zero_()
             raise RuntimeError("a kernel reported: " + ops.describe_device_error(int(picked[R])))
         out = [int(picked[i]) for i in range(n)]
+        if host_rows:                                       # (first: rows that are sent for below come to the same place)
+            picked_host = sample_rows([reqs[i].sampler for i in host_rows], rows_host, [reqs[i].tokens for i in host_rows])
+            for i, tok in zip(host_rows, picked_host):
+                out[i] = tok
         if cand_rows:
             ids, vals, flags = cands
             unsure = [i for j, i in enumerate(cand_rows) if flags[j] or self._distrust_candidates]
@@ -351,19 +374,57 @@ class Engine:
                 more = self._rows_to_host(logits, unsure)
                 torch.cuda.current_stream().synchronize()
                 for i, tok in zip(unsure, sample_rows([reqs[i].sampler for i in unsure], more, [reqs[i].tokens for i in unsure])):
-                    out[i] = tok
+                    out[i] = tok                           # (with the log probabilities, where they are wanted)
             sure = [j for j, i in enumerate(cand_rows) if not (flags[j] or self._distrust_candidates)]
             if sure:
                 rq = [reqs[cand_rows[j]] for j in sure]
                 windows = [r.token_slice(max(0, r.num_tokens - r.params.repeat_last_n), min(r.num_tokens, r.params.repeat_last_n))
                            if r.params.penalizing else [] for r in rq]
-                for j, tok in zip(sure, sample_candidates([r.sampler for r in rq], ids[sure], vals[sure], windows)):
+                for j, tok in zip(sure, sample_candidates([self._drawer(r) for r in rq], ids[sure], vals[sure], windows)):
                     out[cand_rows[j]] = tok
-        if host_rows:
-            picked_host = sample_rows([reqs[i].sampler for i in host_rows], rows_host, [reqs[i].tokens for i in host_rows])
-            for i, tok in zip(host_rows, picked_host):
-                out[i] = tok
+        if prob_rows:
+            logprob, lse, top_ids, top_logprobs = probs
+            place = {i: j for j, i in enumerate(cand_rows)}
+            for q, i in enumerate(prob_rows):
+                value, j = logprob[q], place.get(i)
+                if j is not None:                          # the host has picked: one of the candidates, whose logits are here
+                    if cands[2][j] or self._distrust_candidates:
+                        continue
+                    at = np.nonzero(cands[0][j] == out[i])[0]
+                    value = np.float32(cands[1][j][at[0]] - lse[q]) if at.size else -np.inf
+                n_top = min(reqs[i].params.logprobs, top_ids.shape[1])
+                reqs[i].sampler.probs.append(TokenProbs(out[i], float(value), [(int(a), float(b)) for a, b in zip(top_ids[q, :n_top],
+                                                                                                                  top_logprobs[q, :n_top])]))
         return out
+
+    def _drawer(self, r: Request):
+        """The sampler that draws ``r``'s token.  A request that wants log probabilities would have its whole row brought to the host for them; the device tells
+        them instead (ops.token_logprobs), and the draw goes the way it goes without them: the largest logit, or the host's chain on its candidates.  (A draw
+        from the whole row stays where it was: the device takes a seed's numbers in another order.)"""
+        p, drawer = r.params, r.sampler.drawer
+        told = (p.logprobs is not None and self._narrow_rows and p.logprobs <= ops.TOP_LOGPROBS_MAX
+                and (drawer.params.is_pure_greedy or drawer.candidates_needed > 0))
+        return drawer if told else r.sampler
+
+    def _probs_to_host(self, logits: torch.Tensor, rows: List[int], top: int):
+        """Of each of ``rows``: the log probability of the token that the device has picked, ln sum exp of the raw logits and the ``top`` likeliest tokens,
+        copied to pinned memory (queued; the caller synchronises the stream): logprob, lse, ids, log probabilities as numpy views."""
+        n, cap, top = len(rows), self.runner.R_max, min(top, logits.shape[1])
+        if self._prob_bufs is None or self._prob_bufs[4] < top:
+            words = cap * (2 + 2 * top)
+            self._prob_bufs = (torch.empty(cap, dtype=torch.int32, pin_memory=True), torch.empty((2, cap), dtype=torch.int32, device=self.device),
+                               torch.empty(words, dtype=torch.float32, device=self.device), torch.empty(words, dtype=torch.float32, pin_memory=True), top)
+        idx_host, idx_dev, dev, host, _ = self._prob_bufs
+        idx_host[:n] = torch.as_tensor(rows, dtype=torch.int32)
+        idx, tokens = idx_dev[0, :n], idx_dev[1, :n]
+        idx.copy_(idx_host[:n], non_blocking=True)
+        ops.gather_rows(self._picked_dev.view(-1, 1), idx, tokens.view(-1, 1))
+        ends = [n, 2 * n, (2 + top) * n, (2 + 2 * top) * n]
+        ids = dev[ends[1]:ends[2]].view(torch.int32).view(n, top) if top else None
+        ops.token_logprobs(logits, tokens, dev[:n], lse=dev[n:ends[1]], top_ids=ids, top_logprobs=dev[ends[2]:ends[3]].view(n, top) if top else None, rows=idx)
+        host[:ends[3]].copy_(dev[:ends[3]], non_blocking=True)
+        h = host.numpy()
+        return h[:n], h[n:ends[1]], h[ends[1]:ends[2]].view(np.int32).reshape(n, top), h[ends[2]:ends[3]].reshape(n, top)
 
     def _candidates_to_host(self, logits: torch.Tensor, rows: List[int], n_cand: int):
         """The ``n_cand`` largest logits of each of ``rows`` with their ids, found by the engine's own kernel and
@@ -405,6 +466,86 @@ class Engine:
         ops.gather_rows(logits, idx_dev[:n], dev)
         host[:n].copy_(dev[:n], non_blocking=True)
         return host[:n].numpy()
+
+    # ------------------------------------------------------------ scoring
+    def score(self, prompts: Union[Sequence[int], Sequence[Sequence[int]]], top: int = 0) -> Union[PromptScore, List[PromptScore]]:
+        """Log probabilities of the prompts' own tokens, with the entropies they come from and the ``top`` likeliest tokens at every place, without
+        generating anything: for one prompt (a list of ids) or several, which share steps of up to ``max_batch_tokens``.  The logits are
+        not kept (Head.score).  Between requests only: raises RuntimeError while any is running or waiting."""
+        single = len(prompts) > 0 and not isinstance(prompts[0], (list, tuple, np.ndarray))
+        plist = [[int(t) for t in p] for p in ([prompts] if single else prompts)]
+        V = self.config.vocab_size
+        for p in plist:
+            if not p:
+                raise ValueError("an empty prompt has nothing to score")
+            bad = [t for t in p if not 0 <= t < V]
+            if bad:
+                raise ValueError(f"prompt holds token ids outside [0, {V}): {bad[:5]}")
+            if len(p) - 1 > self.max_context:
+                raise ValueError(f"a prompt of {len(p)} tokens, the context limit is {self.max_context}")
+        if not 0 <= top <= min(ops.TOP_LOGPROBS_MAX, V):
+            raise ValueError(f"top must be from 0 to {min(ops.TOP_LOGPROBS_MAX, V)}")
+        if self.has_work():
+            raise RuntimeError("score() runs between requests, and some are running or waiting")
+        self._ahead = None
+        m, out = self.manager, [PromptScore(p, [None], [None], [[]]) for p in plist]
+        waiting = [i for i, p in enumerate(plist) if len(p) > 1]
+        live: Dict[int, tuple] = {}                        # prompt -> its request
+        done = {i: 0 for i in waiting}                     # tokens that have run
+        try:
+            while waiting or live:
+                while waiting and len(live) < self.runner.R_max:
+                    i = waiting[0]
+                    # as many prompts at a time as the cache holds to their ends
+                    if not m.has_free_slot():
+                        if not live and self.scheduler._drop_kept():
+                            continue
+                        break
+                    rid = ("score", next(self._ids))
+                    m.add_request(rid)
+                    promised: Dict[int, int] = {}
+                    for j, other in live.items():
+                        for g, need in m.pages_needed(other, len(plist[j]) - 1 - done[j]).items():
+                            promised[g] = promised.get(g, 0) + need
+                    if live and not m.can_reserve(rid, len(plist[i]) - 1, promised):
+                        m.free_request(rid)
+                        break
+                    live[i] = rid
+                    waiting.pop(0)
+                if not live:
+                    raise OutOfSlots("no request slot is free for a prompt to score")
+                entries, targets, parts, budget = [], [], [], self.runner.T_max
+                for i, rid in live.items():
+                    n = min(budget, len(plist[i]) - 1 - done[i])
+                    if n == 0:
+                        break
+                    entries.append(StepEntry(rid, plist[i][done[i]:done[i] + n], range(n)))
+                    targets += plist[i][done[i] + 1:done[i] + n + 1]
+                    parts.append((i, n))
+                    budget -= n
+                try:
+                    got = self.runner.score(entries, targets, top)
+                except OutOfPages:
+                    if not self.scheduler._drop_kept():
+                        raise
+                    continue
+                lp, ent = got.logprob.tolist(), got.entropy.tolist()
+                ids, tops = (got.top_ids.tolist(), got.top_logprobs.tolist()) if top else (None, None)
+                at = 0
+                for i, n in parts:
+                    s = out[i]
+                    s.logprobs += lp[at:at + n]
+                    s.entropies += ent[at:at + n]
+                    s.top += [list(zip(ids[q], tops[q])) if top else [] for q in range(at, at + n)]
+                    at += n
+                    done[i] += n
+                    if done[i] == len(plist[i]) - 1:
+                        m.free_request(live.pop(i))
+                self.runner.raise_on_device_error()
+        finally:
+            for rid in live.values():
+                m.free_request(rid)
+        return out[0] if single else out
 
     # ------------------------------------------------------------ generation
     def generate(self, prompts: Union[Sequence[int], Sequence[Sequence[int]]],

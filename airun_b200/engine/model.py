@@ -217,14 +217,16 @@ class DecoderModel:
                 [c.cache_from for c in self.order])
 
     # ---- one pass over the given tokens ----
-    def forward(self, ctx, want_rows: Optional[torch.Tensor], n_want: int) -> Optional[torch.Tensor]:
+    def forward(self, ctx, want_rows: Optional[torch.Tensor], n_want: int, score=None) -> Optional[torch.Tensor]:
+        """Returns float32 logits [n_want, V]; with ``score`` = (tokens int32 [n_want], TokenScores) the wanted rows are scored instead
+        of kept, and nothing is returned."""
         from ..kernels import ops
         T = ctx.num_tokens
         ctx.ws_main.reset()
         x = ctx.ws_main.alloc((T, self.H), torch.float32)
         self.embedding.forward(ctx, ctx.token_ids[:T], x)
         if self.multi_stream:
-            return self._forward_streams(ctx, x, want_rows, n_want)
+            return self._forward_streams(ctx, x, want_rows, n_want, score)
         delta = kept = None
         if self.residual_input is not None:
             ctx.ws = ctx.ws_pair[0]
@@ -275,7 +277,13 @@ class DecoderModel:
                 delta = None
         if delta is not hsel:
             self.final_norm.forward(ctx, x, hsel, delta=delta, rows=want_rows[:n_want])
-        logits = ctx.ws_main.alloc((n_want, self.V), torch.float32)
+        return self._from_head(ctx, hsel, score)
+
+    def _from_head(self, ctx, hsel: torch.Tensor, score) -> Optional[torch.Tensor]:
+        if score is not None:
+            self.head.score(ctx, hsel, *score)
+            return None
+        logits = ctx.ws_main.alloc((hsel.shape[0], self.V), torch.float32)
         self.head.forward(ctx, hsel, logits)
         return logits
 
@@ -293,7 +301,7 @@ class DecoderModel:
             return out
         return x[:T] if pending is None or isinstance(pending, CastActivations) else None
 
-    def _forward_streams(self, ctx, x: torch.Tensor, want_rows: Optional[torch.Tensor], n_want: int) -> Optional[torch.Tensor]:
+    def _forward_streams(self, ctx, x: torch.Tensor, want_rows: Optional[torch.Tensor], n_want: int, score=None) -> Optional[torch.Tensor]:
         """The pass over the layers with a residual of ``streams`` copies, [T, S, H]: every copy starts as the embedding,
         each block leaves its last write pending for the next pass over the streams (parts/block.py:
         HyperConnectionBlock), and the last pass writes it and sums the streams into x for the final norm."""
@@ -324,9 +332,7 @@ class DecoderModel:
         ctx.ws.reset()
         hsel = ctx.ws.alloc((n_want, self.H), self.dtype)
         self.final_norm.forward(ctx, x, hsel, rows=want_rows[:n_want])
-        logits = ctx.ws_main.alloc((n_want, self.V), torch.float32)
-        self.head.forward(ctx, hsel, logits)
-        return logits
+        return self._from_head(ctx, hsel, score)
 
 
 def build_decoder(config: ModelConfig, dtype: torch.dtype, device) -> DecoderModel:

@@ -23,6 +23,7 @@ import torch
 
 from ..cache.manager import CacheManager, CacheStorage, OutOfPages
 from ..kernels import ops
+from ..parts.base import TokenScores
 from .batch import CacheView, StepContext, Workspace
 from .model import DecoderModel
 
@@ -206,6 +207,30 @@ class StepRunner:
         self.manager.commit_many([e.rid for e in entries], [len(e.tokens) for e in entries])
         self.steps_run += 1
         return logits
+
+    def score(self, entries: Sequence[StepEntry], targets: Sequence[int], top: int = 0) -> Optional[TokenScores]:
+        """Runs the entries as one batch like ``step``, but scores the wanted places instead of returning their logits: ``targets`` holds
+        the token asked for at each of them, in the order of the entries and of ``want`` (an id outside the vocabulary asks for none), ``top``
+        how many of the likeliest tokens come along.  Returns TokenScores on the device, or None when nothing is wanted.  Not replayed from
+        a graph: a scored batch is large and comes once."""
+        self.check_entries(entries)
+        n = sum(len(e.want) for e in entries)
+        if len(targets) != n:
+            raise StepError(f"{len(targets)} targets for {n} wanted places")
+        if not 0 <= top <= min(ops.TOP_LOGPROBS_MAX, self.model.V):
+            raise StepError(f"{top} alternatives a place, at most {min(ops.TOP_LOGPROBS_MAX, self.model.V)} can be told")
+        self.reserve(entries)
+        ctx, n_want = self.build_context(entries)
+        scores = None
+        if n:
+            scores = TokenScores.empty(n, top, self.device)
+            tokens = torch.as_tensor(np.asarray(targets, dtype=np.int32)).to(self.device)
+            self.model.forward(ctx, self._view("want_rows"), n_want, score=(tokens, scores))
+        else:
+            self.model.forward(ctx, None, 0)
+        self.manager.commit_many([e.rid for e in entries], [len(e.tokens) for e in entries])
+        self.steps_run += 1
+        return scores
 
     # ---- a step in two halves: what does not depend on the newest tokens, and the rest
     def prepare_step(self, entries: Sequence[StepEntry]) -> Optional[dict]:

@@ -187,11 +187,34 @@ class Embedding(Part):
         raise NotImplementedError
 
 
+@dataclass
+class TokenScores:
+    """What a scored row leaves: the log probability of the token that is asked for, the entropy of the row's distribution (nats) and,
+    where they are wanted, its likeliest tokens with their log probabilities, the best first; float32 and int32 on the device."""
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: Optional[torch.Tensor] = None
+    top_logprobs: Optional[torch.Tensor] = None
+
+    @classmethod
+    def empty(cls, n: int, top: int, device) -> "TokenScores":
+        f = lambda *shape: torch.empty(shape, dtype=torch.float32, device=device)      # noqa: E731
+        return cls(f(n), f(n), torch.empty((n, top), dtype=torch.int32, device=device) if top else None, f(n, top) if top else None)
+
+
 class Head(Part):
-    """forward(ctx, h [rows, hidden] in the compute type, out float32 [rows, vocab])."""
+    """forward(ctx, h [rows, hidden] in the compute type, out float32 [rows, vocab]).
+    score(ctx, h, tokens int32 [rows], scores): log probabilities of the tokens under the rows' distributions; a head that can tell them
+    without the rows' logits has its own."""
 
     def forward(self, ctx, h: torch.Tensor, out: torch.Tensor) -> None:
         raise NotImplementedError
+
+    def score(self, ctx, h: torch.Tensor, tokens: torch.Tensor, scores: TokenScores) -> None:
+        from ..kernels import ops
+        logits = ctx.ws_main.alloc((h.shape[0], self.V), torch.float32)
+        self.forward(ctx, h, logits)
+        ops.token_logprobs(logits, tokens, scores.logprob, scores.entropy, None, scores.top_ids, scores.top_logprobs)
 
 
 class ResidualInput(Part):

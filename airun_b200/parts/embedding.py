@@ -13,7 +13,7 @@ import torch
 
 from ..kernels import ops
 from ..weights.loader import WeightSpec
-from .base import Embedding, Head, register_part
+from .base import Embedding, Head, TokenScores, register_part
 from .linear import linear
 
 
@@ -63,6 +63,10 @@ class LMHead(Head):
             ops.scale_(out, self.scale)
         if self.soft_cap is not None:
             ops.soft_cap(out, self.soft_cap)
+
+    def score(self, ctx, h: torch.Tensor, tokens: torch.Tensor, scores: TokenScores) -> None:
+        ops.head_logprobs(h, self.weight, tokens, scores.logprob, ctx.err, scores.entropy, None, scores.top_ids, scores.top_logprobs,
+                          self.scale, self.soft_cap, ctx.ws)
 
 
 register_part("embedding", "token_embedding", TokenEmbedding)

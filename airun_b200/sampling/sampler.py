@@ -28,7 +28,7 @@ import ctypes
 import itertools
 import math
 import time
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -248,6 +248,11 @@ class Sampler:
         # what the engine asks every step, worked out once (the parameters of a live request do not change)
         self.device_ok = params.device_ok
         self.candidates_needed = params.candidates_needed(512)
+        # who draws when somebody else tells the log probabilities: the same chain and generator without them
+        self.drawer = self
+        if params.logprobs is not None:
+            self.drawer = Sampler(replace(params, logprobs=None))
+            self.drawer.rng = self.rng
 
     def _draw(self, ids: np.ndarray, probs: np.ndarray) -> int:
         """Index into ``ids`` / ``probs`` (descending) of the inverse-CDF draw (sample.rs:478-485)."""
