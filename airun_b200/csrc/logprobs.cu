@@ -181,13 +181,13 @@ template <int NT> __device__ __forceinline__ void rank_top(TopShared<NT>& sh, in
 // The k-th largest of the maxima of groups of threads is a lower bound of the k-th largest of all, and close to it when
 // there are twice as many groups as wanted keys: about k to 2 k keys reach it.  Those are listed and each counts the larger ones.
 // A group is as many lanes as leave 2 k groups, and fewer where logits may come `VEC` neighbours to a thread: equal logits in every place, whose keys
-// fall with the id, list the first vectors of k groups, 512 keys or k NT's least.  A list longer than `few` is cut again in the same way.
+// fall with the id, list the first vectors of k groups, 1,024 keys or those of k threads.  A list longer than `few` is cut again in the same way.
 template <int NT, int VEC, typename Each>
 __device__ __forceinline__ bool select_top(TopShared<NT>& sh, u64 low, u64 high, int k, Each each) {
     constexpr int CAP = TopShared<NT>::CAP, MINE = CAP / NT;
     const int tid = threadIdx.x;
     int g = 32;
-    while (g > 1 && (NT / g < 2 * k || k * g * VEC > 512)) g >>= 1;
+    while (g > 1 && (NT / g < 2 * k || k * g * VEC > 1024)) g >>= 1;
     const int groups = NT / g;
     auto find_cut = [&](u64 b) {
         for (int o = 1; o < g; o <<= 1) {
@@ -301,10 +301,12 @@ template <> struct Pack<__nv_bfloat16> {
 // the threads in batches of U: a thread's elements come by ascending id.  The few elements ahead of the first
 // 16-byte boundary and behind the last belong to the first block's first threads and the last block's first threads.
 // What reaches the bound of the k largest is read again: by few threads, and with C = 1 while the SM's other blocks stream.  TOP: alternatives are wanted.
+// Blocks an SM: three of 512 threads where rows are many, so that some stream while others select (2,048 rows with 20 alternatives 257 us with two, 227); 16
+// logits a batch (bfloat16 in batches of 32 leaves room for two: 333 rows of 50,001 22.8 us, 19.5).
 template <typename T, int NT, bool CLUSTER, bool TOP>
-__global__ __launch_bounds__(NT) void token_logprobs_kernel(const TokenParams p, int n_parts) {
+__global__ __launch_bounds__(NT, NT == 128 ? 8 : CLUSTER ? 2 : 3) void token_logprobs_kernel(const TokenParams p, int n_parts) {
     pdl_trigger();
-    constexpr int VEC = Pack<T>::N, U = 4;
+    constexpr int VEC = Pack<T>::N, U = 16 / VEC;
     __shared__ TopShared<NT> top;
     __shared__ Part s_parts[32];
     __shared__ Part s_part_of[8];                                // of the cluster's blocks, in the first one's memory
@@ -580,7 +582,10 @@ __device__ __forceinline__ float capped(float x, float cap, float over_cap) {
     return cap * (fabsf(z) < 0.25f ? near : fmaf(-2.0f, r, 1.0f));
 }
 
-template <bool PAIR, int TOP>
+// ROLLED: the epilogue's code, which runs once a tile and comes cold, is a quarter as long.  Unrolled it saves the moves, which only pays where tiles follow each
+// other fast: us, rolled and not, 2,048 rows x [151936, 2048] 992, 971; 5 rows x [151936, 4096] with five alternatives 211, 219; 700 rows x [20000, 1024]
+// capped 39, 44.
+template <bool PAIR, int TOP, bool ROLLED>
 __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
     const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const HeadParams p) {
     pdl_trigger();
@@ -759,11 +764,12 @@ __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
                 if (!ok) break;
                 if (!warp_on) continue;
                 const int ids = min(p.bn, t.w_end - w0);           // of this tile
-#pragma unroll
+                // ROLLED: one body, and the next ids are moved up in the registers
+#pragma unroll ROLLED ? 1 : 4
                 for (int j = 0; j < 4; ++j) {
                     const int c = 32 * half + 64 * j, first = w0 + c;
                     if (c >= ids) break;
-                    float (&v)[32] = acc[j];
+                    float (&v)[32] = acc[ROLLED ? 0 : j];
                     if (c + 32 > ids) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) v[i] = c + i < ids ? v[i] : __int_as_float(0x7fffffff);       // no number: nowhere counted
@@ -804,6 +810,12 @@ __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
                             }
                             least = row_on ? list.least(p.k) : INFINITY;
                         }
+                    }
+                    if constexpr (ROLLED) {
+#pragma unroll
+                        for (int a = 0; a < 3; ++a)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) acc[a][i] = acc[a + 1][i];
                     }
                 }
             }
@@ -896,10 +908,10 @@ static int head_map(CUtensorMap* out, const void* ptr, long long rows, long long
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? AIRUN_OK : AIRUN_ERR_ARG;
 }
 
-template <bool PAIR, int TOP>
+template <bool PAIR, int TOP, bool ROLLED>
 static int launch_head(const CUtensorMap& mx, const CUtensorMap& mw, HeadParams p, cudaStream_t stream) {
     static unsigned long long configured = 0;
-    auto kern = head_logprobs_kernel<PAIR, TOP>;
+    auto kern = head_logprobs_kernel<PAIR, TOP, ROLLED>;
     const int w_bytes = p.bn / (PAIR ? 2 : 1) * (BK * 2), x_bytes = p.x_rows * (BK * 2);
     // the products read 128 rows from a stage's first on, in the last one beyond what it brings
     const int beyond = 128 * BK * 2 - x_bytes;
@@ -940,8 +952,10 @@ AIRUN_EXPORT int airun_head_logprobs(const void* x, const void* W, int n, int V,
     HeadParams p = {n, V, K, row_blocks, splits, tiles, bn, part, x_rows, 0, tokens, scale, cap, k, (float*)scratch, nullptr, nullptr, err};
     p.given = p.stats + (size_t)6 * splits * n;
     p.keys = (u64*)((uint8_t*)scratch + ((size_t)4 * (6 * (size_t)splits + 1) * n + 15) / 16 * 16);
-    if (pair) r = k == 0 ? launch_head<true, 0>(mx, mw, p, stream) : k <= 8 ? launch_head<true, 8>(mx, mw, p, stream) : launch_head<true, 16>(mx, mw, p, stream);
-    else r = k == 0 ? launch_head<false, 0>(mx, mw, p, stream) : k <= 8 ? launch_head<false, 8>(mx, mw, p, stream) : launch_head<false, 16>(mx, mw, p, stream);
+#define LAUNCH_HEAD(PAIR, ROLLED) (k == 0 ? launch_head<PAIR, 0, ROLLED>(mx, mw, p, stream) : k <= 8 ? launch_head<PAIR, 8, ROLLED>(mx, mw, p, stream) \
+                                                                                            : launch_head<PAIR, 16, ROLLED>(mx, mw, p, stream))
+    r = !pair ? LAUNCH_HEAD(false, true) : cap > 0.0f ? LAUNCH_HEAD(true, true) : LAUNCH_HEAD(true, false);
+#undef LAUNCH_HEAD
     if (r != AIRUN_OK) return r;
     airun_launch(head_join_kernel, dim3(n), dim3(JOIN_THREADS), 0, stream, (const float*)p.stats, (const float*)p.given, (const u64*)p.keys, tokens, n, V, 2 * splits, k,
                  logprob, entropy, lse, top_ids, top_logprobs);

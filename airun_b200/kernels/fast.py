@@ -391,7 +391,8 @@ HEAD_TOP = 16                          # most alternatives that the fused head k
 def plan_head(n: int, V: int, K: int, sms: int = B200_SMS) -> Tuple[bool, int, int, int, int]:
     """(pairs of SMs, ranges of the vocabulary, tiles of a range, ids of a tile, K-steps of a part of a sum) for the log probabilities of n rows.
 
-    Up to 128 rows an SM to all of them, as the weights' bytes are the bound; sums in parts of 256 values cost nothing there.  Above, by the clocks of
+    Up to 128 rows an SM to all of them, as the weights' bytes are the bound; sums in parts of 256 values cost little there (100 rows with five
+    alternatives 140 us for 133, 5 rows nothing).  Above, by the clocks of
     the rounds that blocks of 128 rows (256 for a pair) and ranges take: 3 an id and K-step, 4 % less on pairs, whose tiles cost 2,500 more
     where K is too short to hide them; 6,000 a range, and 2 % a round for SMs that no longer read the same weights at the same time.  B200, sustained, us,
     pairs and single SMs: 2,048 x 4,096 1,868 and 1,957; 4,095 x 2,048 1,888 and 1,950; 2,048 x 512 309 and 240; with fewer rows
@@ -416,7 +417,7 @@ def plan_head(n: int, V: int, K: int, sms: int = B200_SMS) -> Tuple[bool, int, i
                 best = clocks, pair, ranges, tiles, bn
     if best is None:                                      # more blocks of rows than that: each walks the whole vocabulary
         best = 0, True, 1, (V + 255) // 256, 256
-    return best[1:] + (4 if n <= 128 else 8,)
+    return best[1:] + (4 if n <= 64 else 8,)
 
 
 def head_logprobs_bf16(hidden, weight, tokens, logprob, entropy, lse, top_ids, top_logprobs, scale: float, soft_cap: Optional[float], err,

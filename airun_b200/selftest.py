@@ -750,6 +750,46 @@ def check_group_routing(dev) -> Tuple[float, float]:
     return wrong + _rel(wts, pick.values), 2e-6
 
 
+def ref_logprobs(x: torch.Tensor, tokens: torch.Tensor, k: int):
+    """Log probabilities of the tokens, entropies and the k largest logits' ids (equal ones by ascending id) and log probabilities."""
+    lp = torch.log_softmax(x.double(), dim=-1)
+    ids = torch.from_numpy(np.argsort(-x.double().numpy(), axis=1, kind="stable")[:, :k].copy())
+    return lp.gather(1, tokens.long()[:, None])[:, 0], -torch.special.xlogy(lp.exp(), lp.exp()).sum(1), ids, lp.gather(1, ids)
+
+
+def _logprob_error(got, want) -> float:
+    lp, H, ids, tops = (t.cpu() for t in got)
+    if not torch.equal(ids.long(), want[2]):
+        return float("inf")
+    return max(float(((a.double() - b).abs() / (1 + b.abs())).max()) for a, b in ((lp, want[0]), (H, want[1]), (tops, want[3])))
+
+
+def check_token_logprobs(dev) -> Tuple[float, float]:
+    """A row in parts, rows a block each, a small vocabulary; bfloat16 rows with equal logits."""
+    from .kernels import ops
+    worst = 0.0
+    for n, V, dtype in ((1, 151936, torch.float32), (300, 5000, torch.float32), (64, 384, torch.float32), (40, 20001, torch.bfloat16)):
+        x, k = (3 * torch.randn(n, V)).to(dtype), 7
+        t = torch.randint(0, V, (n,), dtype=torch.int32)
+        out = [torch.empty(n, device=dev), torch.empty(n, device=dev), torch.empty(n, k, dtype=torch.int32, device=dev), torch.empty(n, k, device=dev)]
+        ops.token_logprobs(x.to(dev), t.to(dev), out[0], out[1], None, out[2], out[3])
+        worst = max(worst, _logprob_error(out, ref_logprobs(x, t, k)))
+    return worst, 2e-5
+
+
+def check_head_logprobs(dev) -> Tuple[float, float]:
+    """A few rows, a portion on single SMs and one on pairs, float32; inputs whose products and sums are exact, so that ids are too."""
+    from .kernels import ops
+    worst, err = 0.0, torch.zeros(1, dtype=torch.int32, device=dev)
+    for n, H, V, dtype in ((3, 256, 9000, torch.bfloat16), (150, 1032, 3000, torch.bfloat16), (600, 1024, 5000, torch.bfloat16), (20, 100, 700, torch.float32)):
+        h, w = torch.randint(-4, 5, (n, H)).float() / 4, torch.randint(-8, 9, (V, H)).float() / 64
+        t, k = torch.randint(0, V, (n,), dtype=torch.int32), 4
+        out = [torch.empty(n, device=dev), torch.empty(n, device=dev), torch.empty(n, k, dtype=torch.int32, device=dev), torch.empty(n, k, device=dev)]
+        ops.head_logprobs(h.to(dtype).to(dev), w.to(dtype).to(dev), t.to(dev), out[0], err, out[1], None, out[2], out[3])
+        worst = max(worst, _logprob_error(out, ref_logprobs(h.double() @ w.double().t(), t, k)))
+    return worst + float(err.item()), 2e-5
+
+
 CHECKS: List[Tuple[str, Callable]] = [
     ("embedding gather", check_embedding),
     ("rmsnorm + residual add", check_rmsnorm),
@@ -778,6 +818,8 @@ CHECKS: List[Tuple[str, Callable]] = [
     ("experts chosen in groups by sigmoid scores", check_group_routing),
     ("sampling", check_sampling),
     ("largest logits of a row", check_largest_logits),
+    ("log probabilities from logits", check_token_logprobs),
+    ("log probabilities from hidden states, tcgen05 and float32", check_head_logprobs),
 ]
 
 
