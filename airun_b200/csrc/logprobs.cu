@@ -846,29 +846,29 @@ __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
 
 // The parts of a row become its results: a block a row.  What is in no list is minus infinity (or not a number, which counts as that): where the lists
 // hold fewer than k, the lowest ids that are in none follow.
-#define JOIN_THREADS 128
-__global__ __launch_bounds__(JOIN_THREADS) void head_join_kernel(
+template <int NT>
+__global__ __launch_bounds__(NT) void head_join_kernel(
     const float* stats, const float* given, const u64* keys, const int32_t* tokens, int n, int V, int parts, int k,
     float* logprob, float* entropy, float* lse, int32_t* top_ids, float* top_logprobs) {
     pdl_trigger();
-    __shared__ TopShared<JOIN_THREADS> top;
-    __shared__ Part s_parts[JOIN_THREADS / 32];
+    __shared__ TopShared<NT> top;
+    __shared__ Part s_parts[NT / 32];
     __shared__ Row s_row;
     const int r = blockIdx.x, tid = threadIdx.x;
     pdl_wait();
     Part mine = {-INFINITY, 0.0f, 0.0f};
-    for (int i = tid; i < parts; i += JOIN_THREADS) {
+    for (int i = tid; i < parts; i += NT) {
         const float* at = stats + (size_t)i * n + r;
         mine = join(mine, Part{at[0], at[(size_t)parts * n], at[(size_t)2 * parts * n]});
     }
     if (k > 0) {
         const u64* mine_k = keys + (size_t)r * parts * k;
         u64 best = 0;
-        for (int i = tid; i < parts * k; i += JOIN_THREADS) best = mine_k[i] > best ? mine_k[i] : best;
+        for (int i = tid; i < parts * k; i += NT) best = mine_k[i] > best ? mine_k[i] : best;
         auto each = [&](u64, auto f) {
-            for (int i = tid; i < parts * k; i += JOIN_THREADS) if (mine_k[i]) f(mine_k[i]);
+            for (int i = tid; i < parts * k; i += NT) if (mine_k[i]) f(mine_k[i]);
         };
-        if (!select_top<JOIN_THREADS, 1>(top, best, best, k, each)) one_by_one<JOIN_THREADS>(top, k, each);
+        if (!select_top<NT, 1>(top, best, best, k, each)) one_by_one<NT>(top, k, each);
         if (tid == 0) {
             int at = 0, id = 0;
             while (at < k && top.top[at]) ++at;
@@ -878,7 +878,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void head_join_kernel(
             }
         }
     }
-    const Part all = block_join<JOIN_THREADS>(mine, s_parts);
+    const Part all = block_join<NT>(mine, s_parts);
     if (tid == 0) {
         const Row w = row_of(all);
         const int token = tokens[r];
@@ -889,7 +889,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void head_join_kernel(
     }
     __syncthreads();
     const Row w = s_row;
-    for (int i = tid; i < k; i += JOIN_THREADS) {
+    for (int i = tid; i < k; i += NT) {
         const u64 key = top.top[i];
         top_ids[(size_t)r * k + i] = key_id(key);
         top_logprobs[(size_t)r * k + i] = log_prob(w, key_logit(key));
@@ -957,7 +957,12 @@ AIRUN_EXPORT int airun_head_logprobs(const void* x, const void* W, int n, int V,
     r = !pair ? LAUNCH_HEAD(false, true) : cap > 0.0f ? LAUNCH_HEAD(true, true) : LAUNCH_HEAD(true, false);
 #undef LAUNCH_HEAD
     if (r != AIRUN_OK) return r;
-    airun_launch(head_join_kernel, dim3(n), dim3(JOIN_THREADS), 0, stream, (const float*)p.stats, (const float*)p.given, (const u64*)p.keys, tokens, n, V, 2 * splits, k,
-                 logprob, entropy, lse, top_ids, top_logprobs);
+    const float *stats = p.stats, *given = p.given;
+    const u64* keys = p.keys;
+    // few rows have a part an SM and more; a thread then looks at a few of them
+    if (2 * splits * (k > 0 ? k : 1) > 256)
+        airun_launch(head_join_kernel<512>, dim3(n), dim3(512), 0, stream, stats, given, keys, tokens, n, V, 2 * splits, k, logprob, entropy, lse, top_ids, top_logprobs);
+    else
+        airun_launch(head_join_kernel<128>, dim3(n), dim3(128), 0, stream, stats, given, keys, tokens, n, V, 2 * splits, k, logprob, entropy, lse, top_ids, top_logprobs);
     return airun_launch_status();
 }
