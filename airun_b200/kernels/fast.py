@@ -394,9 +394,9 @@ def plan_head(n: int, V: int, K: int, sms: int = B200_SMS) -> Tuple[bool, int, i
     Up to 128 rows an SM to all of them, as the weights' bytes are the bound; sums in parts of 256 values cost little there (100 rows with five
     alternatives 140 us for 133, 5 rows nothing).  Above, by the clocks of
     the rounds that blocks of 128 rows (256 for a pair) and ranges take: 3 an id and K-step, 4 % less on pairs, whose tiles cost 2,500 more
-    where K is too short to hide them; 6,000 a range, and 2 % a round for SMs that no longer read the same weights at the same time.  B200, sustained, us,
-    pairs and single SMs: 2,048 x 4,096 1,868 and 1,957; 4,095 x 2,048 1,888 and 1,950; 2,048 x 512 309 and 240; with fewer rows
-    that are not there, 300 x 4,096 479 and 376, 640 x 2,048 386 and 294 (151,936 ids all)."""
+    where K is too short to hide them; 6,000 a range, and 5 % a round for SMs that no longer read the same weights at the same time (2,048 x 4,096 on pairs in
+    9, 18 and 46 ranges, one, two and five rounds: 1,596, 1,652 and 1,709).  B200, sustained, us, pairs and single SMs: 2,048 x 4,096 1,868 and 1,957; 4,095 x
+    2,048 1,888 and 1,950; 2,048 x 512 309 and 240; with fewer rows that are not there, 300 x 4,096 479 and 376, 640 x 2,048 386 and 294 (151,936 ids all)."""
     kb = (K + 63) // 64
     best = None
     for pair in (False, True) if n > 128 else (False,):
@@ -412,7 +412,7 @@ def plan_head(n: int, V: int, K: int, sms: int = B200_SMS) -> Tuple[bool, int, i
             ranges = (V + tiles * bn - 1) // (tiles * bn)
             turns = (blocks * ranges + groups - 1) // groups
             tile = kb * bn * 2.9 + (2500 if kb < 16 else 0) if pair else kb * bn * 3.0
-            clocks = turns * (tiles * tile + 6000) * (1 + 0.02 * (turns - 1))
+            clocks = turns * (tiles * tile + 6000) * (1 + 0.05 * (turns - 1))
             if best is None or clocks < best[0]:
                 best = clocks, pair, ranges, tiles, bn
     if best is None:                                      # more blocks of rows than that: each walks the whole vocabulary

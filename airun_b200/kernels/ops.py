@@ -1347,7 +1347,9 @@ def head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tens
 
     ``ws``: an engine.batch.Workspace to take scratch from (None: allocated).  Scratch is in use until the call's kernels are done:
     calls that may overlap on the GPU (two streams, two graphs) need workspaces of their own.  ``err``: int32 [1], the device-side
-    error word."""
+    error word.  Like every product here the kernel may ask for weights while a kernel of this package in front of it still runs: ``weight`` is not
+    written by one of those right before.  Up to 16 alternatives from bfloat16 rows (16-byte aligned, H a multiple of 8) logits exist in tensor memory only;
+    other calls form HEAD_CHUNK of them at a time."""
     _here(hidden, weight, tokens, logprob, err, entropy, lse, top_ids, top_logprobs)
     hs, wsh = hidden.shape, weight.shape
     if len(hs) != 2 or len(wsh) != 2 or hs[1] != wsh[1] or wsh[0] == 0 or wsh[1] == 0:
@@ -1356,14 +1358,21 @@ def head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tens
     _dt(hidden)
     _need(hidden.stride(1) == 1 and weight.stride(1) == 1, "hidden and weight must be row-major")
     n, V = hs[0], wsh[0]
+    _need((n <= 1 or hidden.stride(0) >= hs[1]) and (V <= 1 or weight.stride(0) >= hs[1]), "rows of hidden and weight must not overlap")
     _need(tokens.dim() == 1 and tokens.shape[0] == n, "a token for every row")
     _logprob_outputs(n, V, tokens, logprob, entropy, lse, top_ids, top_logprobs)
     _need(err.dtype == torch.int32 and err.numel() == 1, "err must be one int32")
-    _need(abs(scale) < float("inf"), "the scale must be finite")
-    _need(soft_cap is None or 0.0 < soft_cap < float("inf"), "the cap must be positive")
+    _need(abs(scale) <= 1e30, "the scale must be finite, at most 1e30")
+    _need(soft_cap is None or 1e-30 <= soft_cap <= 1e30, "the cap must be positive, from 1e-30 to 1e30")
     if n == 0:
         return
-    alloc = ws.alloc if ws is not None else (lambda shape, dtype: torch.empty(shape, dtype=dtype, device=hidden.device))
+    def alloc(shape, dtype):
+        if ws is None:
+            return torch.empty(shape, dtype=dtype, device=hidden.device)
+        t = ws.alloc(shape, dtype)
+        _here(t)
+        return t
+
     if hidden.dtype == torch.bfloat16:
         from . import fast
         if fast.head_logprobs_bf16(hidden, weight, tokens, logprob, entropy, lse, top_ids, top_logprobs, scale, soft_cap, err, alloc):

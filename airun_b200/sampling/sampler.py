@@ -248,11 +248,15 @@ class Sampler:
         # what the engine asks every step, worked out once (the parameters of a live request do not change)
         self.device_ok = params.device_ok
         self.candidates_needed = params.candidates_needed(512)
-        # who draws when somebody else tells the log probabilities: the same chain and generator without them
-        self.drawer = self
+        self._drawer = None
         if params.logprobs is not None:
-            self.drawer = Sampler(replace(params, logprobs=None))
-            self.drawer.rng = self.rng
+            self._drawer = Sampler(replace(params, logprobs=None))
+            self._drawer.rng = self.rng
+
+    @property
+    def drawer(self) -> "Sampler":
+        """Who draws when somebody else tells the log probabilities: the same chain and generator without them."""
+        return self._drawer or self
 
     def _draw(self, ids: np.ndarray, probs: np.ndarray) -> int:
         """Index into ``ids`` / ``probs`` (descending) of the inverse-CDF draw (sample.rs:478-485)."""

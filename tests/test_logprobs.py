@@ -348,6 +348,53 @@ def test_head_on_another_stream_and_in_two_graphs(n, V, k):
         assert torch.equal(lp.cpu(), want[0]) and torch.equal(ids.cpu(), want[3]) and torch.equal(tops.cpu(), want[4]) and int(err.item()) == 0
 
 
+@pytest.mark.gpu
+def test_head_sizes_that_fill_rounds_of_blocks_unevenly():
+    """Rows and ids just off the tiles' and ranges' borders, on single SMs and on pairs."""
+    for n, H, V, k in ((129, 64, 2368, 2), (255, 128, 16 * 148 + 1, 3), (385, 1024, 256 * 37 + 1, 2), (513, 64, 255, 4), (1024, 1088, 256 * 18, 0), (1025, 1024, 5000, 16)):
+        h, w = grid_inputs(n, H, V, torch.bfloat16, n)
+        t = some_tokens(n, V, n)
+        got, want = head(h, w, t, k), plain(h.double().cpu() @ w.double().cpu().t(), t.cpu(), k)
+        for g, x in zip(got[:3], want[:3]):
+            near(g, x)
+        assert k == 0 or torch.equal(got[3].long(), want[3]), (n, H, V)
+
+
+@pytest.mark.gpu
+def test_head_calls_on_two_streams_with_workspaces_of_their_own():
+    from airun_b200.engine.batch import Workspace
+    from airun_b200.kernels import ops
+    sets = []
+    for i, (n, V) in enumerate(((70, 9000), (3, 20000))):
+        h, w = grid_inputs(n, 256, V, torch.bfloat16, i)
+        t = some_tokens(n, V, i)
+        sets.append((h, w, t, torch.empty(n, device=DEV), torch.empty(n, 6, dtype=torch.int32, device=DEV), torch.empty(n, 6, device=DEV),
+                     torch.zeros(1, dtype=torch.int32, device=DEV), Workspace(torch.device(DEV), 1 << 20), torch.cuda.Stream(),
+                     plain(h.double().cpu() @ w.double().cpu().t(), t.cpu(), 6)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for h, w, t, lp, ids, tops, err, ws, stream, _ in sets:
+            with torch.cuda.stream(stream):
+                ws.reset()
+                ops.head_logprobs(h, w, t, lp, err, top_ids=ids, top_logprobs=tops, ws=ws)
+    torch.cuda.synchronize()
+    for h, w, t, lp, ids, tops, err, ws, stream, want in sets:
+        near(lp.cpu(), want[0])
+        assert torch.equal(ids.cpu().long(), want[3]) and int(err.item()) == 0
+
+
+def test_plan_of_ranges_covers_the_vocabulary():
+    """Every id lies in one range, no range is empty, tiles have a width the products take."""
+    import random
+    from airun_b200.kernels.fast import plan_head
+    rng = random.Random(1)
+    for _ in range(3000):
+        n, V, K = int(2 ** rng.uniform(0, 18)), int(2 ** rng.uniform(0, 18)), 8 * int(2 ** rng.uniform(0, 10))
+        pair, ranges, tiles, bn, part = plan_head(n, V, K, rng.choice((148, 132, 20, 2)))
+        assert ranges * tiles * bn >= V > (ranges - 1) * tiles * bn and 16 <= bn <= 256 and bn % (32 if pair else 16) == 0 and part in (4, 8), (n, V, K)
+        assert not pair or n > 128
+
+
 class _Fake:
     """A tensor's stand-in that says it is on the GPU, for the checks that come before any launch."""
 
@@ -406,6 +453,10 @@ def test_head_refusals(monkeypatch):
     refused("together", top_logprobs=_Fake(4, 3))
     refused("to the vocabulary", top_ids=_Fake(4, 101, dtype=torch.int32), top_logprobs=_Fake(4, 101))
     refused("int32", err=_Fake(1))
-    refused("finite", scale=float("nan"))
-    refused("positive", soft_cap=0.0)
+    refused("overlap", hidden=_Fake(64).as_strided((4, 64), (0, 1)))
+    refused("overlap", weight=_Fake(6400).as_strided((100, 64), (32, 1)))
+    for scale in (float("nan"), float("inf"), 1e39):
+        refused("finite", scale=scale)
+    for cap in (0.0, -1.0, 1e-50, 1e39, float("nan")):
+        refused("positive", soft_cap=cap)
     refused("dtype", hidden=_Fake(4, 64, dtype=torch.float16), weight=_Fake(100, 64, dtype=torch.float16))
