@@ -391,8 +391,8 @@ HEAD_TOP = 16                          # most alternatives that the fused head k
 def plan_head(n: int, V: int, K: int, sms: int = B200_SMS) -> Tuple[bool, int, int, int, int]:
     """(pairs of SMs, ranges of the vocabulary, tiles of a range, ids of a tile, K-steps of a part of a sum) for the log probabilities of n rows.
 
-    Up to 128 rows an SM to all of them, as the weights' bytes are the bound; sums in parts of 256 values cost little there (100 rows with five
-    alternatives 140 us for 133, 5 rows nothing).  Above, by the clocks of
+    Up to 128 rows an SM to all of them, as the weights' bytes are the bound; up to 64 sums in parts of 128 values cost nothing (5 rows
+    x 4,096 184 us for 187 in parts of 512, entropies off by 0.8e-6 for 2.2e-6), 100 rows with five alternatives take 140 us for 133.  Above, by the clocks of
     the rounds that blocks of 128 rows (256 for a pair) and ranges take: 3 an id and K-step, 4 % less on pairs, whose tiles cost 2,500 more
     where K is too short to hide them; 6,000 a range, and 5 % a round for SMs that no longer read the same weights at the same time (2,048 x 4,096 on pairs in
     9, 18 and 46 ranges, one, two and five rounds: 1,596, 1,652 and 1,709).  B200, sustained, us, pairs and single SMs: 2,048 x 4,096 1,868 and 1,957; 4,095 x
@@ -417,7 +417,7 @@ def plan_head(n: int, V: int, K: int, sms: int = B200_SMS) -> Tuple[bool, int, i
                 best = clocks, pair, ranges, tiles, bn
     if best is None:                                      # more blocks of rows than that: each walks the whole vocabulary
         best = 0, True, 1, (V + 255) // 256, 256
-    return best[1:] + (4 if n <= 64 else 8,)
+    return best[1:] + (2 if n <= 64 else 8,)
 
 
 def head_logprobs_bf16(hidden, weight, tokens, logprob, entropy, lse, top_ids, top_logprobs, scale: float, soft_cap: Optional[float], err,

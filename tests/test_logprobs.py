@@ -391,7 +391,7 @@ def test_plan_of_ranges_covers_the_vocabulary():
     for _ in range(3000):
         n, V, K = int(2 ** rng.uniform(0, 18)), int(2 ** rng.uniform(0, 18)), 8 * int(2 ** rng.uniform(0, 10))
         pair, ranges, tiles, bn, part = plan_head(n, V, K, rng.choice((148, 132, 20, 2)))
-        assert ranges * tiles * bn >= V > (ranges - 1) * tiles * bn and 16 <= bn <= 256 and bn % (32 if pair else 16) == 0 and part in (4, 8), (n, V, K)
+        assert ranges * tiles * bn >= V > (ranges - 1) * tiles * bn and 16 <= bn <= 256 and bn % (32 if pair else 16) == 0 and part in (2, 8), (n, V, K)
         assert not pair or n > 128
 
 
