@@ -846,7 +846,37 @@ __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
     }
 }
 
-// The parts of a row become its results: a block a row.  What is in no list is minus infinity (or not a number, which counts as that): where the lists
+// The parts of a row become its results.  Without alternatives by warps.
+__device__ __forceinline__ Part part_at(const float* stats, int i, int parts, int n, int r) {
+    const float* at = stats + (size_t)i * n + r;
+    return {at[0], at[(size_t)parts * n], at[(size_t)2 * parts * n]};
+}
+__device__ __forceinline__ Row write_row(const Part& all, const float* given, int token, int V, int r, float* logprob, float* entropy, float* lse) {
+    const Row w = row_of(all);
+    logprob[r] = token >= 0 && token < V ? log_prob(w, given[r]) : -INFINITY;
+    if (lse) lse[r] = row_lse(w);
+    if (entropy) entropy[r] = w.entropy;
+    return w;
+}
+
+template <int ROWS>                                                // of a block of 128 threads: 4, or 1 where rows are few and have many parts
+__global__ __launch_bounds__(128) void head_rows_kernel(
+    const float* stats, const float* given, const int32_t* tokens, int n, int V, int parts, float* logprob, float* entropy, float* lse) {
+    pdl_trigger();
+    __shared__ Part s_parts[4];
+    constexpr int THREADS = 128 / ROWS;
+    const int r = blockIdx.x * ROWS + threadIdx.x / THREADS, at = threadIdx.x % THREADS;
+    pdl_wait();
+    Part mine = {-INFINITY, 0.0f, 0.0f};
+    if (r < n) {
+#pragma unroll 4
+        for (int i = at; i < parts; i += THREADS) mine = join(mine, part_at(stats, i, parts, n, r));
+    }
+    mine = ROWS == 1 ? block_join<128>(mine, s_parts) : warp_join(mine);
+    if (r < n && at == 0) write_row(mine, given, tokens[r], V, r, logprob, entropy, lse);
+}
+
+// With alternatives a block a row.  What is in no list is minus infinity (or not a number, which counts as that): where the lists
 // hold fewer than k, the lowest ids that are in none follow.
 template <int NT>
 __global__ __launch_bounds__(NT) void head_join_kernel(
@@ -859,36 +889,24 @@ __global__ __launch_bounds__(NT) void head_join_kernel(
     const int r = blockIdx.x, tid = threadIdx.x;
     pdl_wait();
     Part mine = {-INFINITY, 0.0f, 0.0f};
-    for (int i = tid; i < parts; i += NT) {
-        const float* at = stats + (size_t)i * n + r;
-        mine = join(mine, Part{at[0], at[(size_t)parts * n], at[(size_t)2 * parts * n]});
-    }
-    if (k > 0) {
-        const u64* mine_k = keys + (size_t)r * parts * k;
-        u64 best = 0;
-        for (int i = tid; i < parts * k; i += NT) best = mine_k[i] > best ? mine_k[i] : best;
-        auto each = [&](u64, auto f) {
-            for (int i = tid; i < parts * k; i += NT) if (mine_k[i]) f(mine_k[i]);
-        };
-        if (!select_top<NT, 1>(top, best, best, k, each)) one_by_one<NT>(top, k, each);
-        if (tid == 0) {
-            int at = 0, id = 0;
-            while (at < k && top.top[at]) ++at;
-            for (const int found = at; at < k; ++at, ++id) {
-                for (int j = 0; j < found; ++j) if (key_id(top.top[j]) == id) { ++id; j = -1; }
-                top.top[at] = key_of(-INFINITY, id);
-            }
+    for (int i = tid; i < parts; i += NT) mine = join(mine, part_at(stats, i, parts, n, r));
+    const u64* mine_k = keys + (size_t)r * parts * k;
+    u64 best = 0;
+    for (int i = tid; i < parts * k; i += NT) best = mine_k[i] > best ? mine_k[i] : best;
+    auto each = [&](u64, auto f) {
+        for (int i = tid; i < parts * k; i += NT) if (mine_k[i]) f(mine_k[i]);
+    };
+    if (!select_top<NT, 1>(top, best, best, k, each)) one_by_one<NT>(top, k, each);
+    if (tid == 0) {
+        int at = 0, id = 0;
+        while (at < k && top.top[at]) ++at;
+        for (const int found = at; at < k; ++at, ++id) {
+            for (int j = 0; j < found; ++j) if (key_id(top.top[j]) == id) { ++id; j = -1; }
+            top.top[at] = key_of(-INFINITY, id);
         }
     }
     const Part all = block_join<NT>(mine, s_parts);
-    if (tid == 0) {
-        const Row w = row_of(all);
-        const int token = tokens[r];
-        s_row = w;
-        logprob[r] = token >= 0 && token < V ? log_prob(w, given[r]) : -INFINITY;
-        if (lse) lse[r] = row_lse(w);
-        if (entropy) entropy[r] = w.entropy;
-    }
+    if (tid == 0) s_row = write_row(all, given, tokens[r], V, r, logprob, entropy, lse);
     __syncthreads();
     const Row w = s_row;
     for (int i = tid; i < k; i += NT) {
@@ -962,7 +980,11 @@ AIRUN_EXPORT int airun_head_logprobs(const void* x, const void* W, int n, int V,
     const float *stats = p.stats, *given = p.given;
     const u64* keys = p.keys;
     // few rows have a part an SM and more; a thread then looks at a few of them
-    if (2 * splits * (k > 0 ? k : 1) > 256)
+    if (k == 0 && 2 * splits > 64)
+        airun_launch(head_rows_kernel<1>, dim3(n), dim3(128), 0, stream, stats, given, tokens, n, V, 2 * splits, logprob, entropy, lse);
+    else if (k == 0)
+        airun_launch(head_rows_kernel<4>, dim3((n + 3) / 4), dim3(128), 0, stream, stats, given, tokens, n, V, 2 * splits, logprob, entropy, lse);
+    else if (2 * splits * k > 256)
         airun_launch(head_join_kernel<512>, dim3(n), dim3(512), 0, stream, stats, given, keys, tokens, n, V, 2 * splits, k, logprob, entropy, lse, top_ids, top_logprobs);
     else
         airun_launch(head_join_kernel<128>, dim3(n), dim3(128), 0, stream, stats, given, keys, tokens, n, V, 2 * splits, k, logprob, entropy, lse, top_ids, top_logprobs);
