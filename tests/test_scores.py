@@ -74,6 +74,38 @@ def test_scored_places_agree_with_their_logits(name, dtype, folders):
     eng.runner.raise_on_device_error()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("design,shape", [("losalorn", "l1"), ("losalorn", "l2"), ("tagulix", "t1"), ("tagulix", "t4"), ("gamanex", "g1")])
+def test_other_designs_are_scored(design, shape, dtype, tmp_path):
+    """A capped head, a residual of several streams, a head of a model with its own norm: portions of two requests against the step's logits."""
+    import importlib
+    from airun_b200 import Engine, StepEntry
+    t = importlib.import_module("test_" + design)
+    make, page = t.SHAPES[shape][:2]
+    cfg = make()
+    more = {"rel_rows": t.SHAPES[shape][2]} if len(t.SHAPES[shape]) > 2 else {}
+    folder = t.P.write_folder(str(tmp_path), cfg, t.P.random_weights(cfg, seed=5, **more))
+    eng = Engine.from_folder(folder, dtype=dtype, page_size=page, cache_tokens=512, max_batch_tokens=128, max_requests=4, max_context=512)
+    V = eng.config.vocab_size
+    toks = [random_tokens(n, V, n) for n in (30, 13)]
+    entries = [StepEntry(r, s, range(len(s))) for r, s in zip("ab", toks)]
+    targets = [x for s in toks for x in s[1:] + s[:1]]
+
+    def fresh():
+        for r in "ab":
+            if r in eng.manager.requests:
+                eng.manager.free_request(r)
+            eng.manager.add_request(r)
+
+    fresh()
+    lp, H, all_lp = from_logits(eng.runner.step(entries).float().cpu(), targets)
+    fresh()
+    got = eng.runner.score(entries, targets, 3)
+    eng.runner.raise_on_device_error()
+    assert float((got.logprob.cpu().double() - lp).abs().max()) < TOL and float((got.entropy.cpu().double() - H).abs().max()) < TOL
+    assert float((got.top_logprobs.cpu().double() - all_lp.gather(1, got.top_ids.cpu().long())).abs().max()) < TOL
+
+
 def test_score_refuses_what_step_refuses(folders):
     from airun_b200 import StepEntry
     from airun_b200.engine.step import StepError
