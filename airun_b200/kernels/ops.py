@@ -45,9 +45,10 @@ def _p(t: Optional[torch.Tensor]):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)     # of a device; current_stream() makes an object of it, 4 us
 
 
-def _stream() -> c_void_p:
+def _stream(device: Optional[int] = None) -> c_void_p:
+    """The current stream (``device``: the current device, where the caller has asked for it already)."""
     if _raw_stream is not None:
-        return c_void_p(_raw_stream(torch.cuda.current_device()))
+        return c_void_p(_raw_stream(torch.cuda.current_device() if device is None else device))
     return c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
@@ -62,13 +63,14 @@ def _cuda(*ts: Optional[torch.Tensor]) -> None:
             _need(t.is_cuda, "kernel arguments must live on the GPU (there is no CPU path)")
 
 
-def _here(*ts: Optional[torch.Tensor]) -> None:
-    """All on the current device, whose stream the kernel is launched on."""
+def _here(*ts: Optional[torch.Tensor]) -> int:
+    """All on the current device, whose stream the kernel is launched on; returns that device."""
     here = torch.cuda.current_device()
     for t in ts:
         if t is not None and t.get_device() != here:
             _cuda(t)
             raise KernelError("kernel arguments must live on the current device")
+    return here
 
 
 def _at(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -1316,7 +1318,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Te
     entropy 0, one with plus infinity the entropy NaN; a token outside [0, V) has minus infinity, so rows that are padding may ask for
     -1.  A row index outside [0, R) reads nothing: it gives what a row without a distribution does, with ids of -1, and sets
     the bit of a bad row in ``err``, if that is given."""
-    _here(logits, tokens, logprob, entropy, lse, top_ids, top_logprobs, rows, err)
+    device = _here(logits, tokens, logprob, entropy, lse, top_ids, top_logprobs, rows, err)
     shape, n = logits.shape, tokens.shape[0]
     if len(shape) != 2 or shape[1] == 0 or logits.stride(1) != 1:
         raise KernelError("logits must be row-major [rows, V]")
@@ -1330,7 +1332,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Te
     _need(ld >= V, "rows of logits must not overlap")
     f = _fn("logprobs", "airun_token_logprobs", _TOKEN_LOGPROBS)
     _check(f(logits.data_ptr(), _dt(logits), ld, R, V, _at(rows), tokens.data_ptr(), n, logprob.data_ptr(), _at(entropy), _at(lse), k, _at(top_ids),
-             _at(top_logprobs), _at(err), _stream()), "token_logprobs")
+             _at(top_logprobs), _at(err), _stream(device)), "token_logprobs")
 
 
 _TOKEN_LOGPROBS = [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
