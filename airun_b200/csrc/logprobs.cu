@@ -785,7 +785,7 @@ __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
 #pragma unroll
                         for (int i = 0; i < 32; ++i) v[i] = capped(v[i], p.cap, over_cap);
                     }
-                    if (token >= first && token < min(first + 32, t.w_end)) {
+                    if (token >= first && token < min(first + 32, w0 + ids)) {      // (a tile may end inside the 32, and the next one begins there)
                         float x = v[0];
 #pragma unroll
                         for (int i = 1; i < 32; ++i) x = token == first + i ? v[i] : x;

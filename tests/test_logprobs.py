@@ -361,6 +361,29 @@ def test_head_sizes_that_fill_rounds_of_blocks_unevenly():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,V,k", [(40, 70000, 16), (128, 70000, 8), (40, 70000, 0)])
+def test_head_tiles_that_end_inside_a_warps_ids(n, V, k):
+    """Tiles of 240 ids, whose last 16 share 32 columns with what lies behind: tokens at the start of the next tile belong to other warps, which come there early
+    where every id of the one enters its lists and none of the other's does."""
+    from airun_b200.kernels.fast import plan_head
+    pair, ranges, tiles, bn, _ = plan_head(n, V, 64)
+    assert not pair and tiles > 1 and bn % 64 == 48
+    place = torch.arange(V) % (tiles * bn)
+    late = place % bn // 32 % 2 == 1
+    g = torch.Generator().manual_seed(7)
+    h, w = torch.zeros(n, 64, dtype=torch.bfloat16), torch.randint(-8, 9, (V, 64), generator=g).to(torch.bfloat16) / 64
+    h[:, 0], h[:, 1] = 1.0, torch.arange(n) % 5 / 4
+    w[:, 0] = torch.where(late, (place // 2).float() / 16, torch.tensor(-4.0)).to(torch.bfloat16)
+    first = torch.randint(0, ranges - 1, (n,), generator=g) * tiles * bn + bn
+    t = (first + torch.randint(0, 16, (n,), generator=g)).to(torch.int32).to(DEV)
+    want, got = plain(h.double() @ w.double().t(), t.cpu(), k), head(h.to(DEV), w.to(DEV), t, k)
+    for a, b in zip(got[:3], want[:3]):
+        near(a, b)
+    if k:
+        assert torch.equal(got[3].long(), want[3])
+
+
+@pytest.mark.gpu
 def test_head_calls_on_two_streams_with_workspaces_of_their_own():
     from airun_b200.engine.batch import Workspace
     from airun_b200.kernels import ops
