@@ -671,7 +671,12 @@ __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
             // the last commits arrive at this CTA's barriers before it may leave
             for (int i = max(0, it - stages); i < it && ok; ++i)
                 ok = mbar_wait_warp(empty + 8 * (i % stages), (i / stages) & 1);
-            if (!ok) atomicOr(p.err, AIRUN_DEV_TIMEOUT);
+            if (!ok) {
+                atomicOr(p.err, AIRUN_DEV_TIMEOUT);
+                // what is on its way lands before the memory is given up (a pair's loads all tell the leader, and both leave together)
+                for (int i = max(0, it - stages); i < it && rank == 0; ++i)
+                    if (!mbar_wait_warp(full + 8 * (i % stages), (i / stages) & 1)) break;
+            }
         } else if (warp == 1 && rank == 0) {
             const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(128 * CTAS >> 4) << 24);
             int n = 0;                                             // sums so far
@@ -728,7 +733,7 @@ __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
                 float acc[4][32];                                  // ids 32 half + 64 j and 31 more
                 for (int kb = 0; kb < kb_total; kb += p.part, ++n) {
                     const int buf = n & 1;
-                    ok = mbar_wait(accf + 8 * buf, (n >> 1) & 1);
+                    ok = mbar_wait_warp(accf + 8 * buf, (n >> 1) & 1);
                     if (!ok) { atomicOr(p.err, AIRUN_DEV_TIMEOUT); break; }
                     tc_fence_after();
                     __syncwarp();
