@@ -19,7 +19,10 @@ typedef unsigned long long u64;
 // ------------------------------------------------------------------ parts of a row
 #define LOWEST (-200.0f)               // exp is 0 from here on, and so is a term's part in u
 
-struct Part { float m, s, u; };
+// A part's s without the 1 that its maximum stands for: where one token leads, s is 1 and a little, and each addition would round the little, and with it the
+// entropy, to 2^-24 of the 1.  Entropies of 300 single rows of 151,936: relative errors up to 5e-7, 0.9e-7 in the mean square; 10e-7 and 1.5e-7 with s itself;
+// joined in 64 bits 5e-7 and 0.9e-7, but 7.2 us a row for 6.9.
+struct Part { float m, rest, u; };
 
 __device__ __forceinline__ float exp_of(float d) {
     float e;
@@ -31,7 +34,8 @@ __device__ __forceinline__ float below(float x, float m) { return fmaxf(x - m, L
 
 __device__ __forceinline__ Part join(const Part& a, const Part& b) {
     const float m = fmaxf(a.m, b.m), da = below(a.m, m), db = below(b.m, m), fa = exp_of(da), fb = exp_of(db);
-    return {m, fa * a.s + fb * b.s, fa * fmaf(da, a.s, a.u) + fb * fmaf(db, b.s, b.u)};
+    const float ra = fmaf(fa, a.rest, fa), rb = fmaf(fb, b.rest, fb);
+    return {m, a.m >= b.m ? a.rest + rb : ra + b.rest, fa * a.u + da * ra + (fb * b.u + db * rb)};
 }
 
 // A part that grows, chunk by chunk.  A chunk's sums start at zero and join the others with what the additions before have rounded
@@ -39,7 +43,7 @@ __device__ __forceinline__ Part join(const Part& a, const Part& b) {
 // are off by 3e-6, as much as the logits of a head of 4,096 values.
 struct Run {
     float m = -INFINITY, s = 0.0f, u = 0.0f, s_lost = 0.0f, u_lost = 0.0f;
-    __device__ __forceinline__ Part part() const { return {m, s, u}; }
+    __device__ __forceinline__ Part part() const { return {m, (s - 1.0f) - s_lost, u}; }
 };
 
 __device__ __forceinline__ void add_to(float& sum, float& lost, float x) {
@@ -109,8 +113,9 @@ template <int N> __device__ __forceinline__ float most_of(const float (&x)[N]) {
 }
 
 __device__ __forceinline__ Part warp_join(const Part& p) {
-    const float m = warp_max(p.m), d = below(p.m, m), f = exp_of(d);
-    return {m, warp_sum(f * p.s), warp_sum(f * fmaf(d, p.s, p.u))};
+    const float m = warp_max(p.m), d = below(p.m, m), f = exp_of(d), r = fmaf(f, p.rest, f);
+    const bool first = (int)(threadIdx.x & 31) == __ffs(__ballot_sync(0xffffffffu, p.m == m)) - 1;
+    return {m, warp_sum(first ? p.rest : r), warp_sum(fmaf(f, p.u, d * r))};
 }
 
 // The joined part of the block's threads, in its first warp.  `sh` holds one Part a warp.
@@ -129,8 +134,8 @@ struct Row { float m, ln_s, entropy; };
 __device__ __forceinline__ Row row_of(const Part& p) {
     if (p.m == -INFINITY) return {p.m, -INFINITY, 0.0f};
     if (p.m == INFINITY) return {p.m, 0.0f, __int_as_float(0x7fffffff)};
-    const float ln_s = logf(p.s);
-    return {p.m, ln_s, ln_s - p.u / p.s};
+    const float ln_s = log1pf(p.rest);
+    return {p.m, ln_s, ln_s - p.u / (1.0f + p.rest)};
 }
 __device__ __forceinline__ float log_prob(const Row& r, float x) {
     return x > -INFINITY && r.m > -INFINITY ? (x - r.m) - r.ln_s : -INFINITY;
@@ -418,7 +423,7 @@ __global__ __launch_bounds__(NT, NT == 128 ? 8 : CLUSTER ? 2 : 3) void token_log
         if (tid == 0) {
             const uint32_t to = map_to_cta((uint32_t)__cvta_generic_to_shared(&s_part_of[part]), 0);
             asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(all.m) : "memory");
-            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(all.s) : "memory");
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(all.rest) : "memory");
             asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(all.u) : "memory");
         }
         if constexpr (TOP) {
@@ -525,7 +530,7 @@ struct HeadParams {
     const int32_t* tokens;
     float scale, cap;
     int k;
-    float* stats;                                                  // [3][2 splits][n]: m, s, u
+    float* stats;                                                  // [3][2 splits][n]: m, s - 1, u
     float* given;                                                  // [n] logits of the given tokens
     u64* keys;                                                     // [n][2 splits][k]
     int* err;
@@ -831,7 +836,7 @@ __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
                 const int parts = 2 * p.splits, part = 2 * (u / p.row_blocks) + half;
                 float* to = p.stats + (size_t)part * p.n + row;
                 to[0] = mine.m;
-                to[(size_t)parts * p.n] = mine.s;
+                to[(size_t)parts * p.n] = mine.part().rest;
                 to[(size_t)2 * parts * p.n] = mine.u;
                 if constexpr (TOP > 0) {
                     u64* keys = p.keys + ((size_t)row * parts + part) * p.k;
