@@ -510,7 +510,7 @@ AIRUN_EXPORT int airun_token_logprobs(const void* logits, int dtype, long long l
 //   PAIR   : two SMs to 256 rows, tcgen05.mma.cta_group::2 with M = 256; each brings 128 rows and half of the ids, 32 KB a K-step of 64
 //            values, which is what 512 clocks of products leave time for.  What prompts run on.
 //   !PAIR  : an SM to 128 rows, of which only `x_rows` are brought (what the products read behind them ends in lanes nobody looks at): up
-//            to 128 rows are bound by the weights' bytes.
+//            to 128 rows are bound by the weights' bytes.  (Up to 32 rows head_few_kernel takes.)
 //   warp 0    : TMA loads into a ring of stages; asks for weights, which no kernel writes, ahead of the wait for the kernel in front;
 //   warp 1    : allocates tensor memory, issues the products (in a pair, the leader's);
 //   warps 4-11: epilogue, two warps a quadrant of lanes, every other 32 ids of a tile; they take the registers of the first four.
@@ -1000,4 +1000,193 @@ AIRUN_EXPORT int airun_head_logprobs(const void* x, const void* W, int n, int V,
     else
         airun_launch(head_join_kernel<128>, dim3(n), dim3(128), 0, stream, stats, given, keys, tokens, n, V, 2 * splits, k, logprob, entropy, lse, top_ids, top_logprobs);
     return airun_launch_status();
+}
+
+// ------------------------------------------------------------------ from hidden states, few rows
+// Up to 32 rows the ids are the M side of the product and the rows its N side: an SM multiplies 16 or 32 columns where head_logprobs_kernel multiplies 128 rows
+// whatever is in them, and its power goes into bytes.  The logits of a few rows are little beside the weights (4 n V bytes for 2 K V): they are written, and
+// token_logprobs_kernel takes them from the L2.  A block walks a range of the vocabulary in tiles of `bn` <= 128 ids, of any number, so that the ranges come
+// out even.  us, this and head_logprobs_kernel: 5 rows x [151936, 4096] 188, 209, with five alternatives 195, 220; 16 rows 196, 216; 24 rows 200, 211; 32 rows
+// 214, 215, with eight alternatives 222, 234; 5 rows x [20000, 1024] 12.3, 14.2; 32 rows x [384, 64] 5.8, 5.0.
+//   warp 0: TMA loads; warp 1: tensor memory, products; warps 2-5: the sums of a quadrant of lanes each, one id a thread.
+// A stage is FEW_K K-steps, and its sums two parts of 128 values in neighbouring columns that are loaded together: a load takes 1,100 clocks
+// whatever its width.  (Stages of one K-step 237 us for 5 rows, of two 197.)
+#define FEW_THREADS 192
+#define FEW_STAGES 16                                              // at most
+#define FEW_BUFS 4
+#define FEW_K 4
+
+struct FewParams {
+    int n, V, K, tiles, bn;
+    int w_stride, x_bytes, stages;                                 // bytes of a K-step; stages
+    float scale, cap;
+    float* logits;
+    long long ld;
+    int* err;
+};
+
+template <int N>
+__global__ __launch_bounds__(FEW_THREADS, 1) void head_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const FewParams p) {
+    pdl_trigger();
+    __shared__ __align__(8) uint64_t bars[2 * FEW_STAGES + 2 * FEW_BUFS];
+    __shared__ uint32_t tmem_slot;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+    constexpr int COLS = N * (FEW_K / 2);                        // of a buffer: the parts of a stage
+    const int kb_total = (p.K + FEW_K * BK - 1) / (FEW_K * BK), stages = p.stages;
+    const int first_id = blockIdx.x * p.tiles * p.bn, end_id = min(p.V, first_id + p.tiles * p.bn);
+    const uint32_t w_at = smem_u32(smem), x_at = w_at + stages * FEW_K * p.w_stride;
+    const uint32_t full = smem_u32(bars), empty = full + 8 * FEW_STAGES, accf = empty + 8 * FEW_STAGES, acce = accf + 8 * FEW_BUFS;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < FEW_STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
+        for (int b = 0; b < FEW_BUFS; ++b) { mbar_init(accf + 8 * b, 1); mbar_init(acce + 8 * b, 4); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), FEW_BUFS * COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const int n_steps = (end_id - first_id + p.bn - 1) / p.bn * kb_total, first_n = min(n_steps, stages);
+    const uint32_t bytes = FEW_K * (p.bn * (BK * 2) + p.x_bytes);
+    bool ok = true;
+    if (warp == 0) {
+        auto load_w = [&](int s, int kb, int w0) {
+            mbar_expect_tx(full + 8 * s, bytes);
+#pragma unroll
+            for (int a = 0; a < FEW_K; ++a) tma_load_2d(w_at + (FEW_K * s + a) * p.w_stride, &map_w, full + 8 * s, (FEW_K * kb + a) * BK, w0);
+        };
+        if (elect_one()) {                                         // weights: no kernel writes them
+            for (int it = 0, kb = 0, w0 = first_id; it < first_n; ++it) {
+                load_w(it, kb, w0);
+                if (++kb == kb_total) { kb = 0; w0 += p.bn; }
+            }
+        }
+        __syncwarp();
+        pdl_wait();
+        int it = 0, s = 0, kb = 0, w0 = first_id;
+        uint32_t phase = 0;
+        for (; it < n_steps; ++it) {
+            if (it >= first_n && !mbar_wait_warp(empty + 8 * s, phase ^ 1)) { ok = false; break; }
+            if (elect_one()) {
+                if (it >= first_n) load_w(s, kb, w0);
+#pragma unroll
+                for (int a = 0; a < FEW_K; ++a) tma_load_2d(x_at + (FEW_K * s + a) * p.x_bytes, &map_x, full + 8 * s, (FEW_K * kb + a) * BK, 0);
+            }
+            __syncwarp();
+            if (++s == stages) { s = 0; phase ^= 1; }
+            if (++kb == kb_total) { kb = 0; w0 += p.bn; }
+        }
+        // the last commits arrive at the barriers, and where a wait has run out the loads on their way land, before the block may leave
+        const uint32_t last = ok ? empty : full;
+        if (!ok) atomicOr(p.err, AIRUN_DEV_TIMEOUT);
+        for (int i = max(0, it - stages); i < it; ++i)
+            if (!mbar_wait_warp(last + 8 * (i % stages), (i / stages) & 1)) { atomicOr(p.err, AIRUN_DEV_TIMEOUT); break; }
+    } else if (warp == 1) {
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+        int s = 0;
+        uint32_t phase = 0;
+        for (int n = 0; n < n_steps; ++n) {
+            const int buf = n % FEW_BUFS;
+            ok = mbar_wait_warp(acce + 8 * buf, ((n / FEW_BUFS) & 1) ^ 1) && mbar_wait_warp(full + 8 * s, phase);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+                for (int a = 0; a < FEW_K; ++a) {
+                    const uint64_t dw = smem_desc_sw128(w_at + (FEW_K * s + a) * p.w_stride), dx = smem_desc_sw128(x_at + (FEW_K * s + a) * p.x_bytes);
+#pragma unroll
+                    for (int k = 0; k < BK / 16; ++k) umma_bf16(tmem + buf * COLS + a / 2 * N, dw + (uint64_t)(k * 2), dx + (uint64_t)(k * 2), idesc, a % 2 > 0 || k > 0 ? 1u : 0u);
+                }
+                umma_commit(empty + 8 * s);
+                umma_commit(accf + 8 * buf);
+            }
+            __syncwarp();
+            if (++s == stages) { s = 0; phase ^= 1; }
+        }
+        if (!ok) atomicOr(p.err, AIRUN_DEV_TIMEOUT);
+    } else {
+        const int quad = warp & 3;
+        int n = 0;
+        const float over_cap = 1.0f / p.cap;
+        pdl_wait();                                                // the logits' place may be in use
+        for (int w0 = first_id; w0 < end_id && ok; w0 += p.bn) {
+            float acc[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+            for (int kb = 0; kb < kb_total; ++kb, ++n) {
+                const int buf = n % FEW_BUFS;
+                ok = mbar_wait_warp(accf + 8 * buf, (n / FEW_BUFS) & 1);
+                if (!ok) { atomicOr(p.err, AIRUN_DEV_TIMEOUT); break; }
+                tc_fence_after();
+                uint32_t a[COLS];
+#pragma unroll
+                for (int i = 0; i < COLS; i += 32) tmem_ld32_async(tmem + buf * COLS + i + ((uint32_t)(quad * 32) << 16), a + i);
+#pragma unroll
+                for (int i = 0; i < COLS; i += 32) tmem_wait32(a + i);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(acce + 8 * buf) : "memory");
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) acc[i % N] += __uint_as_float(a[i]);
+            }
+            const int i = quad * 32 + lane;
+            if (ok && i < min(p.bn, end_id - w0)) {
+                float* to = p.logits + w0 + i;
+#pragma unroll
+                for (int r = 0; r < N; ++r) {
+                    if (r < p.n) {
+                        float x = acc[r];
+                        if (p.scale != 1.0f) x *= p.scale;
+                        if (p.cap > 0.0f) x = capped(x, p.cap, over_cap);
+                        to[r * p.ld] = x;
+                    }
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, FEW_BUFS * COLS);
+    }
+}
+
+template <int N>
+static int launch_few(const CUtensorMap& mx, const CUtensorMap& mw, FewParams p, cudaStream_t stream) {
+    static unsigned long long configured = 0;
+    auto kern = head_few_kernel<N>;
+    // the products read 128 ids and N rows from a stage's first on, in the last ones beyond what they bring
+    const int beyond_x = N * BK * 2 - p.x_bytes, beyond_w = 128 * BK * 2 - p.w_stride;
+    p.stages = (HEAD_SMEM - 1024 - beyond_x - beyond_w) / (FEW_K * (p.w_stride + p.x_bytes));
+    if (p.stages > FEW_STAGES) p.stages = FEW_STAGES;
+    const int smem = 1024 + p.stages * FEW_K * (p.w_stride + p.x_bytes) + beyond_x + beyond_w;
+    if (first_on_device(configured)) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, HEAD_SMEM);
+        if (e != cudaSuccess) { configured = 0; return (int)e; }
+    }
+    airun_launch(kern, dim3((p.V + p.tiles * p.bn - 1) / (p.tiles * p.bn)), dim3(FEW_THREADS), smem, stream, mx, mw, p);
+    return airun_launch_status();
+}
+
+// x, W and the results as above, n <= 32, k <= TOP_MAX; the vocabulary in ranges of `tiles` tiles of `bn` ids; logits: [n][ld] float32.
+AIRUN_EXPORT int airun_head_few(const void* x, const void* W, int n, int V, int K, long long ldx, long long ldw, const int32_t* tokens, float scale, float cap,
+                                int tiles, int bn, float* logits, long long ld, float* logprob, float* entropy, float* lse, int k, int32_t* top_ids,
+                                float* top_logprobs, int* err, cudaStream_t stream) {
+    if (n <= 0 || n > 32 || V <= 0 || V > 0x7fff0000 || K <= 0 || K % 8 || ldx < K || ldw < K || ldx % 8 || ldw % 8 || ((uintptr_t)x | (uintptr_t)W) & 15) return AIRUN_ERR_ARG;
+    if (!tokens || !logprob || k < 0 || k > TOP_MAX || k > V || (k > 0 && (!top_ids || !top_logprobs))) return AIRUN_ERR_ARG;
+    if (!x || !W || !logits || !err || ld < V || bn < 1 || bn > 128 || tiles < 1 || (long long)tiles * bn > 0x3fffffff) return AIRUN_ERR_ARG;
+    if ((long long)V + (long long)tiles * bn > 0x7fff0000 || (long long)tiles * ((K + BK - 1) / BK) > 0x3fffffff) return AIRUN_ERR_ARG;
+    CUtensorMap mx, mw;
+    const int x_rows = (n + 7) / 8 * 8;
+    int r;
+    if ((r = head_map(&mx, x, n, K, ldx, x_rows)) != AIRUN_OK) return r;
+    if ((r = head_map(&mw, W, V, K, ldw, bn)) != AIRUN_OK) return r;
+    const FewParams p = {n, V, K, tiles, bn, (bn + 7) / 8 * 8 * (BK * 2), x_rows * (BK * 2), 0, scale, cap, logits, ld, err};
+    if ((r = n <= 16 ? launch_few<16>(mx, mw, p, stream) : launch_few<32>(mx, mw, p, stream)) != AIRUN_OK) return r;
+    return airun_token_logprobs(logits, AIRUN_DT_F32, ld, n, V, nullptr, tokens, n, logprob, entropy, lse, k, top_ids, top_logprobs, nullptr, stream);
 }

@@ -391,7 +391,7 @@ HEAD_TOP = 16                          # most alternatives that the fused head k
 def plan_head(n: int, V: int, K: int, sms: int = B200_SMS) -> Tuple[bool, int, int, int, int]:
     """(pairs of SMs, ranges of the vocabulary, tiles of a range, ids of a tile, K-steps of a part of a sum) for the log probabilities of n rows.
 
-    Up to 128 rows an SM to all of them, as the weights' bytes are the bound; up to 64 sums in parts of 128 values cost nothing (5 rows
+    Up to 128 rows an SM to all of them, as the weights' bytes are the bound; up to 64 sums in parts of 128 values cost nothing (few rows
     x 4,096 184 us for 187 in parts of 512, entropies off by 0.8e-6 for 2.2e-6), 100 rows with five alternatives take 140 us for 133.  Above, by the clocks of
     the rounds that blocks of 128 rows (256 for a pair) and ranges take: 3 an id and K-step, 4 % less on pairs, whose tiles cost 2,500 more
     where K is too short to hide them; 6,000 a range, and 5 % a round for SMs that no longer read the same weights at the same time (2,048 x 4,096 on pairs in
@@ -420,25 +420,45 @@ def plan_head(n: int, V: int, K: int, sms: int = B200_SMS) -> Tuple[bool, int, i
     return best[1:] + (2 if n <= 64 else 8,)
 
 
+HEAD_FEW = 32                          # most rows whose logits are written (both forms' times stand at head_few_kernel)
+
+
+def plan_few(V: int, sms: int = B200_SMS) -> Tuple[int, int]:
+    """(tiles of a range, ids of a tile): a range of the vocabulary an SM, in even tiles of up to 128 ids."""
+    per = (V + sms - 1) // sms
+    tiles = (per + 127) // 128
+    return tiles, max(8, (per + tiles - 1) // tiles)
+
+
 def head_logprobs_bf16(hidden, weight, tokens, logprob, entropy, lse, top_ids, top_logprobs, scale: float, soft_cap: Optional[float], err,
                        alloc) -> bool:
-    """``ops.head_logprobs`` in one kernel that forms the logits in tensor memory, and one that joins its parts; False where it does not take the
-    sizes.  ``alloc``: gives scratch, as a Workspace's does."""
+    """``ops.head_logprobs`` in two kernels: up to HEAD_FEW rows one that forms the logits and ``token_logprobs`` of them, above one that forms them in tensor
+    memory and one that joins its parts; False where they do not take the sizes.  ``alloc``: gives scratch, as a Workspace's does."""
     n, K = hidden.shape
     V = weight.shape[0]
     k = 0 if top_ids is None else top_ids.shape[1]
-    if "head_logprobs" in DISABLED or not _usable(hidden, weight) or k > HEAD_TOP:
+    if "head_logprobs" in DISABLED or not _usable(hidden, weight):
+        return False
+    at, ldx, ldw = ops._at, hidden.stride(0) if n > 1 else max(K, hidden.stride(0)), weight.stride(0) if V > 1 else max(K, weight.stride(0))
+    if n <= HEAD_FEW:
+        tiles, bn = plan_few(V, machine(hidden.device).sms)
+        logits = alloc((n, (V + 3) // 4 * 4), torch.float32)
+        f = _fn("logprobs", "airun_head_few", _HEAD_FEW)
+        _check(f(hidden.data_ptr(), weight.data_ptr(), n, V, K, ldx, ldw, tokens.data_ptr(), scale, soft_cap or 0.0, tiles, bn, logits.data_ptr(),
+                 logits.shape[1], logprob.data_ptr(), at(entropy), at(lse), k, at(top_ids), at(top_logprobs), err.data_ptr(), _stream()), "head_logprobs")
+        return True
+    if k > HEAD_TOP:
         return False
     pair, splits, tiles, bn, part = plan_head(n, V, K, machine(hidden.device).sms)
     scratch = alloc(((4 * (6 * splits + 1) * n + 15) // 16 * 16 + 16 * splits * n * k,), torch.uint8)
     f = _fn("logprobs", "airun_head_logprobs", _HEAD_LOGPROBS)
-    at = ops._at
-    _check(f(hidden.data_ptr(), weight.data_ptr(), n, V, K, hidden.stride(0) if n > 1 else max(K, hidden.stride(0)),
-             weight.stride(0) if V > 1 else max(K, weight.stride(0)), tokens.data_ptr(), scale, soft_cap or 0.0, 1 if pair else 0, splits, tiles, bn, part,
+    _check(f(hidden.data_ptr(), weight.data_ptr(), n, V, K, ldx, ldw, tokens.data_ptr(), scale, soft_cap or 0.0, 1 if pair else 0, splits, tiles, bn, part,
              scratch.data_ptr(), logprob.data_ptr(), at(entropy), at(lse), k, at(top_ids), at(top_logprobs), err.data_ptr(), _stream()), "head_logprobs")
     return True
 
 
+_HEAD_FEW = [c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_void_p, c_float, c_float, c_int, c_int, c_void_p, c_longlong, c_void_p,
+             c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p]
 _HEAD_LOGPROBS = [c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_void_p, c_float, c_float, c_int, c_int, c_int, c_int, c_int, c_void_p,
                   c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p]
 

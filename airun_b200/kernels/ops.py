@@ -1345,13 +1345,13 @@ def head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tens
                   entropy: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, top_ids: Optional[torch.Tensor] = None,
                   top_logprobs: Optional[torch.Tensor] = None, scale: float = 1.0, soft_cap: Optional[float] = None, ws=None) -> None:
     """``token_logprobs`` of the logits hidden @ weight^T, times ``scale`` and capped to soft_cap * tanh(logits / soft_cap), without a
-    place for them: hidden [n, H] and weight [V, H], both float32 or both bfloat16, row-major; the other arguments as there.
+    place of theirs: hidden [n, H] and weight [V, H], both float32 or both bfloat16, row-major; the other arguments as there.
 
     ``ws``: an engine.batch.Workspace to take scratch from (None: allocated).  Scratch is in use until the call's kernels are done:
     calls that may overlap on the GPU (two streams, two graphs) need workspaces of their own.  ``err``: int32 [1], the device-side
     error word.  Like every product here the kernel may ask for weights while a kernel of this package in front of it still runs: ``weight`` is not
-    written by one of those right before.  Up to 16 alternatives from bfloat16 rows (16-byte aligned, H a multiple of 8) logits exist in tensor memory only;
-    other calls form HEAD_CHUNK of them at a time."""
+    written by one of those right before.  From bfloat16 rows (16-byte aligned, H a multiple of 8) up to 32 have their logits in scratch, more than those with
+    up to 16 alternatives in tensor memory only; other calls form HEAD_CHUNK of them at a time."""
     _here(hidden, weight, tokens, logprob, err, entropy, lse, top_ids, top_logprobs)
     hs, wsh = hidden.shape, weight.shape
     if len(hs) != 2 or len(wsh) != 2 or hs[1] != wsh[1] or wsh[0] == 0 or wsh[1] == 0:

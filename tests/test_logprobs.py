@@ -384,6 +384,64 @@ def test_head_tiles_that_end_inside_a_warps_ids(n, V, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,H,V,k", [(1, 8, 1, 1), (1, 64, 129, 128), (9, 520, 1184, 20), (15, 136, 18944, 0), (16, 1032, 18945, 128), (17, 256, 7, 7), (24, 264, 37889, 5),
+                                     (25, 72, 2049, 17), (31, 4104, 1300, 3), (32, 512, 50001, 16)])
+def test_head_few_rows(n, H, V, k):
+    """Ranges and tiles of every kind: one id, odd ones, last tiles and K-steps that are partly or wholly outside; the same bits again."""
+    h, w = grid_inputs(n, H, V, torch.bfloat16, n * H + V)
+    h[n // 2] = 0
+    t = some_tokens(n, V, n)
+    got, again = head(h, w, t, k, 0.5, 2.0), head(h, w, t, k, 0.5, 2.0)
+    x = 2.0 * torch.tanh(0.5 * (h.double().cpu() @ w.double().cpu().t()) / 2.0)
+    want = plain(x, t.cpu(), k)
+    for a, b in zip(got[:3], want[:3]):
+        near(a, b)
+    if k:
+        near(got[4], want[4])
+        plainly = head(h, w, t, k)
+        exact = plain(h.double().cpu() @ w.double().cpu().t(), t.cpu(), k)
+        assert torch.equal(plainly[3].long(), exact[3])
+        near(plainly[4], exact[4])
+    for a, b in zip(got, again):
+        assert a is None or torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_head_few_and_more_rows_agree():
+    """The last rows of the one form and the first of the other: the same rows, alone and among others."""
+    h, w = grid_inputs(33, 1024, 9001, torch.bfloat16, 11)
+    t = some_tokens(33, 9001, 3)
+    few, more = head(h[:32], w, t[:32], 5), head(h, w, t, 5)
+    for a, b in zip(few[:3], more[:3]):
+        near(a, b[:32].double())
+    assert torch.equal(few[3], more[3][:32])
+
+
+@pytest.mark.gpu
+def test_head_few_rows_far_into_a_large_vocabulary():
+    """Rows of a strided weight past 2^31 elements; the last ids lead."""
+    V, H = 300000, 64
+    buf = torch.zeros(V, 8192, dtype=torch.bfloat16, device=DEV)
+    w = buf[:, 8000:8000 + H]
+    g = torch.Generator().manual_seed(5)
+    w.copy_((torch.randint(-8, 9, (V, H), generator=g).float() / 64).to(torch.bfloat16))
+    h, _ = grid_inputs(6, H, 8, torch.bfloat16, 6)
+    t = torch.tensor([0, V - 1, V - 2, V, -1, 149999], dtype=torch.int32, device=DEV)
+    want, got = plain(h.double().cpu() @ w.double().cpu().t(), t.cpu(), 4), head(h, w, t, 4)
+    for a, b in zip(got[:3], want[:3]):
+        near(a, b)
+    assert torch.equal(got[3].long(), want[3])
+
+
+def test_plan_of_few_rows_covers_the_vocabulary():
+    from airun_b200.kernels.fast import plan_few
+    for V in list(range(1, 2500)) + [18944, 18945, 32000, 151936, 262144, 1 << 20]:
+        for sms in (148, 132, 2):
+            tiles, bn = plan_few(V, sms)
+            assert 8 <= bn <= 128 and tiles >= 1 and -(-V // (tiles * bn)) <= sms, (V, sms)
+
+
+@pytest.mark.gpu
 def test_head_calls_on_two_streams_with_workspaces_of_their_own():
     from airun_b200.engine.batch import Workspace
     from airun_b200.kernels import ops
