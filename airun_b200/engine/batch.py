@@ -36,7 +36,7 @@ class Workspace:
         n = 1
         for s in shape:
             n *= int(s)
-        esz = torch.empty((), dtype=dtype).element_size()
+        esz = dtype.itemsize
         nbytes = max(n * esz, 1)
         need = (nbytes + self.ALIGN - 1) // self.ALIGN * self.ALIGN
         while True:

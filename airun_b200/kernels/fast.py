@@ -442,10 +442,11 @@ def head_logprobs_bf16(hidden, weight, tokens, logprob, entropy, lse, top_ids, t
     at, ldx, ldw = ops._at, hidden.stride(0) if n > 1 else max(K, hidden.stride(0)), weight.stride(0) if V > 1 else max(K, weight.stride(0))
     if n <= HEAD_FEW:
         tiles, bn = plan_few(V, machine(hidden.device).sms)
-        logits = alloc((n, (V + 3) // 4 * 4), torch.float32)
+        ld = (V + 3) // 4 * 4
+        logits = alloc((4 * n * ld,), torch.uint8)
         f = _fn("logprobs", "airun_head_few", _HEAD_FEW)
         _check(f(hidden.data_ptr(), weight.data_ptr(), n, V, K, ldx, ldw, tokens.data_ptr(), scale, soft_cap or 0.0, tiles, bn, logits.data_ptr(),
-                 logits.shape[1], logprob.data_ptr(), at(entropy), at(lse), k, at(top_ids), at(top_logprobs), err.data_ptr(), _stream()), "head_logprobs")
+                 ld, logprob.data_ptr(), at(entropy), at(lse), k, at(top_ids), at(top_logprobs), err.data_ptr(), _stream()), "head_logprobs")
         return True
     if k > HEAD_TOP:
         return False
