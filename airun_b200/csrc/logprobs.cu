@@ -1007,10 +1007,12 @@ AIRUN_EXPORT int airun_head_logprobs(const void* x, const void* W, int n, int V,
 // whatever is in them, and its power goes into bytes.  The logits of a few rows are little beside the weights (4 n V bytes for 2 K V): they are written, and
 // token_logprobs_kernel takes them from the L2.  A block walks a range of the vocabulary in tiles of `bn` <= 128 ids, of any number, so that the ranges come
 // out even.  us, this and head_logprobs_kernel: 5 rows x [151936, 4096] 188, 209, with five alternatives 195, 220; 16 rows 196, 216; 24 rows 200, 211; 32 rows
-// 214, 215, with eight alternatives 222, 234; 5 rows x [20000, 1024] 12.3, 14.2; 32 rows x [384, 64] 5.8, 5.0.
+// 214, 215, with eight alternatives 222, 234; 5 rows x [20000, 1024] 12.9, 14.2; 32 rows x [384, 64] 5.8, 5.0.
 //   warp 0: TMA loads; warp 1: tensor memory, products; warps 2-5: the sums of a quadrant of lanes each, one id a thread.
-// A stage is FEW_K K-steps, and its sums two parts of 128 values in neighbouring columns that are loaded together: a load takes 1,100 clocks
-// whatever its width.  (Stages of one K-step 237 us for 5 rows, of two 197.)
+// A stage is FEW_K K-steps, and its sums are parts of 64 values (128 for more than 16 rows) in neighbouring columns that are loaded together: a load takes 1,100
+// clocks whatever its width.  (Stages of one K-step 237 us for 5 rows, of two 197.)  The stages' sums are added with compensation: entropies of 5 rows x 4,096
+// off by 3.1e-7 in the mean square, by 7.8e-7 in parts of 128 without it (float32 products of cuBLAS 6.6e-7), 188.5 us for 187.6; 5 rows
+// x [20000, 1024] 12.9 us for 12.2.
 #define FEW_THREADS 192
 #define FEW_STAGES 16                                              // at most
 #define FEW_BUFS 4
@@ -1033,7 +1035,8 @@ __global__ __launch_bounds__(FEW_THREADS, 1) void head_few_kernel(const __grid_c
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
-    constexpr int COLS = N * (FEW_K / 2);                        // of a buffer: the parts of a stage
+    constexpr int PART = N == 16 ? 1 : 2;                          // K-steps of a part
+    constexpr int COLS = N * (FEW_K / PART);                        // of a buffer: the parts of a stage
     const int kb_total = (p.K + FEW_K * BK - 1) / (FEW_K * BK), stages = p.stages;
     const int first_id = blockIdx.x * p.tiles * p.bn, end_id = min(p.V, first_id + p.tiles * p.bn);
     const uint32_t w_at = smem_u32(smem), x_at = w_at + stages * FEW_K * p.w_stride;
@@ -1098,7 +1101,7 @@ __global__ __launch_bounds__(FEW_THREADS, 1) void head_few_kernel(const __grid_c
                 for (int a = 0; a < FEW_K; ++a) {
                     const uint64_t dw = smem_desc_sw128(w_at + (FEW_K * s + a) * p.w_stride), dx = smem_desc_sw128(x_at + (FEW_K * s + a) * p.x_bytes);
 #pragma unroll
-                    for (int k = 0; k < BK / 16; ++k) umma_bf16(tmem + buf * COLS + a / 2 * N, dw + (uint64_t)(k * 2), dx + (uint64_t)(k * 2), idesc, a % 2 > 0 || k > 0 ? 1u : 0u);
+                    for (int k = 0; k < BK / 16; ++k) umma_bf16(tmem + buf * COLS + a / PART * N, dw + (uint64_t)(k * 2), dx + (uint64_t)(k * 2), idesc, a % PART > 0 || k > 0 ? 1u : 0u);
                 }
                 umma_commit(empty + 8 * s);
                 umma_commit(accf + 8 * buf);
@@ -1113,9 +1116,9 @@ __global__ __launch_bounds__(FEW_THREADS, 1) void head_few_kernel(const __grid_c
         const float over_cap = 1.0f / p.cap;
         pdl_wait();                                                // the logits' place may be in use
         for (int w0 = first_id; w0 < end_id && ok; w0 += p.bn) {
-            float acc[N];
+            float acc[N], lost[N];                                 // (compensated as a row's sums are)
 #pragma unroll
-            for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+            for (int i = 0; i < N; ++i) acc[i] = lost[i] = 0.0f;
             for (int kb = 0; kb < kb_total; ++kb, ++n) {
                 const int buf = n % FEW_BUFS;
                 ok = mbar_wait_warp(accf + 8 * buf, (n / FEW_BUFS) & 1);
@@ -1130,7 +1133,13 @@ __global__ __launch_bounds__(FEW_THREADS, 1) void head_few_kernel(const __grid_c
                 __syncwarp();
                 if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(acce + 8 * buf) : "memory");
 #pragma unroll
-                for (int i = 0; i < COLS; ++i) acc[i % N] += __uint_as_float(a[i]);
+                for (int i = 0; i < N; ++i) {
+                    float sum = __uint_as_float(a[i]);
+#pragma unroll
+                    for (int j = N; j < COLS; j += N) sum += __uint_as_float(a[i + j]);
+                    add_to(acc[i], lost[i], sum);
+                    if (!(fabsf(lost[i]) < INFINITY)) lost[i] = 0.0f;        // (a sum that is infinite stays so)
+                }
             }
             const int i = quad * 32 + lane;
             if (ok && i < min(p.bn, end_id - w0)) {

@@ -407,6 +407,24 @@ def test_head_few_rows(n, H, V, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 20])
+def test_head_few_rows_infinite_logits_stay_so(n):
+    """An infinite product early in a sum, with parts behind it; of both signs: no number."""
+    h, w = grid_inputs(n, 1024, 700, torch.bfloat16, 21)
+    h[:, 3], h[:, 900] = 1.0, 1.0
+    w[5, 3], w[6, 3], w[7, 900] = math.inf, -math.inf, -math.inf
+    w[8, 3], w[8, 900] = -math.inf, math.inf
+    t = torch.tensor([5, 6, 8] + [9] * (n - 3), dtype=torch.int32, device=DEV)
+    got = head(h, w, t, 2)
+    assert bool((got[2] == math.inf).all()) and bool(torch.isnan(got[1]).all()) and bool((got[3][:, 0] == 5).all())
+    w[5, 3] = 0.0
+    want, got = plain(h.double().cpu() @ w.double().cpu().t(), t.cpu(), 3), head(h, w, t, 3)
+    for a, b in zip(got[:3], want[:3]):
+        near(a, b)
+    assert got[0][1] == -math.inf and got[0][2] == -math.inf and torch.equal(got[3].long(), want[3])
+
+
+@pytest.mark.gpu
 def test_head_few_and_more_rows_agree():
     """The last rows of the one form and the first of the other: the same rows, alone and among others."""
     h, w = grid_inputs(33, 1024, 9001, torch.bfloat16, 11)
