@@ -1054,21 +1054,21 @@ __global__ __launch_bounds__(FEW_THREADS, 1) void head_few_kernel(const __grid_c
     const uint32_t tmem = tmem_slot;
     const int n_steps = (end_id - first_id + p.bn - 1) / p.bn * kb_total, first_n = min(n_steps, stages);
     const uint32_t bytes = FEW_K * (p.bn * (BK * 2) + p.x_bytes);
+    auto load_w = [&](int s, int kb, int w0) {
+        mbar_expect_tx(full + 8 * s, bytes);
+#pragma unroll
+        for (int a = 0; a < FEW_K; ++a) tma_load_2d(w_at + (FEW_K * s + a) * p.w_stride, &map_w, full + 8 * s, (FEW_K * kb + a) * BK, w0);
+    };
+    if (warp == 0 && elect_one()) {                                // weights: no kernel writes them
+        for (int it = 0, kb = 0, w0 = first_id; it < first_n; ++it) {
+            load_w(it, kb, w0);
+            if (++kb == kb_total) { kb = 0; w0 += p.bn; }
+        }
+    }
+    __syncwarp();
+    pdl_wait();                                                    // all warps: the waits below are bounded, the kernel in front is not
     bool ok = true;
     if (warp == 0) {
-        auto load_w = [&](int s, int kb, int w0) {
-            mbar_expect_tx(full + 8 * s, bytes);
-#pragma unroll
-            for (int a = 0; a < FEW_K; ++a) tma_load_2d(w_at + (FEW_K * s + a) * p.w_stride, &map_w, full + 8 * s, (FEW_K * kb + a) * BK, w0);
-        };
-        if (elect_one()) {                                         // weights: no kernel writes them
-            for (int it = 0, kb = 0, w0 = first_id; it < first_n; ++it) {
-                load_w(it, kb, w0);
-                if (++kb == kb_total) { kb = 0; w0 += p.bn; }
-            }
-        }
-        __syncwarp();
-        pdl_wait();
         int it = 0, s = 0, kb = 0, w0 = first_id;
         uint32_t phase = 0;
         for (; it < n_steps; ++it) {
@@ -1114,7 +1114,6 @@ __global__ __launch_bounds__(FEW_THREADS, 1) void head_few_kernel(const __grid_c
         const int quad = warp & 3;
         int n = 0;
         const float over_cap = 1.0f / p.cap;
-        pdl_wait();                                                // the logits' place may be in use
         for (int w0 = first_id; w0 < end_id && ok; w0 += p.bn) {
             float acc[N], lost[N];                                 // (compensated as a row's sums are)
 #pragma unroll

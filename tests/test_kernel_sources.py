@@ -64,3 +64,18 @@ def test_kernels_wait_before_they_end_and_trigger_first():
         launched = set(re.findall(r"\bairun_launch\w*\(\(*(\w+?)(?:<|,)", text))
         assert launched <= seen | {"kern", "KERNEL", "kernel"}, (name, launched - seen)
     assert {"gemm_pair_kernel", "gemm_tcgen05_kernel", "gemm_rows_kernel", "delta_chunk_kernel"} <= seen
+
+
+def test_bounded_waits_come_behind_the_wait_for_the_kernel_in_front():
+    """A wait on a barrier gives up after two seconds, but the kernel in front may run for longer: a warp that stood at a barrier meanwhile, for operands that another
+    warp asks for behind its pdl_wait(), would report a wait that has run out.  In the kernels of log probabilities every warp passes pdl_wait() first, once and for
+    all roles."""
+    text, seen = SOURCES["logprobs.cu"], 0
+    for at in re.finditer(r"__global__[^;{]*?\bvoid\s+(\w+)\s*\(", text):
+        end = text.find("\n}\n", at.end())
+        body = text[at.end():end]
+        assert body.count("pdl_wait();") == 1 and re.search(r"^    pdl_wait\(\);", body, re.M), at.group(1)
+        front = body[:body.index("pdl_wait();")]
+        assert "mbar_wait" not in front and "mbar_try_wait" not in front, at.group(1)
+        seen += "mbar_wait" in body
+    assert seen == 2
