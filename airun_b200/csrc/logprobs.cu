@@ -40,10 +40,11 @@ __device__ __forceinline__ Part join(const Part& a, const Part& b) {
 
 // A part that grows, chunk by chunk.  A chunk's sums start at zero and join the others with what the additions before have rounded
 // away (compensated summation, W. Kahan, Communications of the ACM 8, 1965): beside one leading token, 8,000 terms of 1e-6 added one by one
-// are off by 3e-6, as much as the logits of a head of 4,096 values.
+// are off by 3e-6, as much as the logits of a head of 4,096 values.  The maximum's 1 is in no running sum either, whether it comes early or late (an entropy from a
+// second token of probability 3e-8 was off by 5 % where the leading one came later).
 struct Run {
-    float m = -INFINITY, s = 0.0f, u = 0.0f, s_lost = 0.0f, u_lost = 0.0f;
-    __device__ __forceinline__ Part part() const { return {m, (s - 1.0f) - s_lost, u}; }
+    float m = -INFINITY, rest = 0.0f, u = 0.0f, rest_lost = 0.0f, u_lost = 0.0f;
+    __device__ __forceinline__ Part part() const { return {m, rest - rest_lost, u}; }
 };
 
 __device__ __forceinline__ void add_to(float& sum, float& lost, float x) {
@@ -74,14 +75,20 @@ __device__ __forceinline__ u64 mul_pair(u64 a, u64 b) {
     return r;
 }
 
-// N logits, of which none is larger than `most`.  Two at a time: additions and products take half the issue slots that way.
-template <int N> __device__ __forceinline__ void add_chunk(Run& r, const float (&x)[N], float most) {
-    if (most > r.m) {
+// What the chunk with the maximum adds up to is rounded to 2^-24 of its 1.  Where less than this is left of a whole row without the 1, the chunk is looked at
+// again (others_again).  Not so where logits are formed and used at once: to keep 32 of them until then costs 6 % of 2,048 rows x [151936, 512], and what is rounded
+// is the probability of the 31 ids beside the leading one, by less than the logits' own errors from a width of 512 on.
+#define FEW_OTHERS 0.0625f
+
+// N logits, of which none is larger than `most`; true where they have brought the maximum.  Two at a time: additions and products take half the issue slots that way.
+template <int N> __device__ __forceinline__ bool add_chunk(Run& r, const float (&x)[N], float most) {
+    const bool moved = most > r.m;
+    if (moved) {
         const float d = below(r.m, most), f = exp_of(d);
-        r.u = f * fmaf(d, r.s, r.u);
-        r.u_lost = f * fmaf(d, r.s_lost, r.u_lost);
-        r.s *= f;
-        r.s_lost *= f;
+        r.u = f * fmaf(d, 1.0f + r.rest, r.u);
+        r.u_lost = f * fmaf(d, r.rest_lost, r.u_lost);
+        r.rest = fmaf(f, r.rest, f);
+        r.rest_lost *= f;
         r.m = most;
     }
     const u64 minus_m = pair_of(-r.m, -r.m), log2_e = pair_of(1.4426950408889634f, 1.4426950408889634f);
@@ -100,9 +107,12 @@ template <int N> __device__ __forceinline__ void add_chunk(Run& r, const float (
     }
     float a, b;
     of_pair(s, a, b);
-    add_to(r.s, r.s_lost, a + b);
+    float sum = a + b;
+    if (moved) sum -= 1.0f;
+    add_to(r.rest, r.rest_lost, sum);
     of_pair(u, a, b);
     add_to(r.u, r.u_lost, a + b);
+    return moved;
 }
 
 template <int N> __device__ __forceinline__ float most_of(const float (&x)[N]) {
@@ -112,10 +122,29 @@ template <int N> __device__ __forceinline__ float most_of(const float (&x)[N]) {
     return most == most ? most : -INFINITY;                        // (all of them not numbers)
 }
 
-__device__ __forceinline__ Part warp_join(const Part& p) {
+// `leader`: the first lane that has the maximum.
+__device__ __forceinline__ Part warp_join(const Part& p, int& leader) {
     const float m = warp_max(p.m), d = below(p.m, m), f = exp_of(d), r = fmaf(f, p.rest, f);
-    const bool first = (int)(threadIdx.x & 31) == __ffs(__ballot_sync(0xffffffffu, p.m == m)) - 1;
-    return {m, warp_sum(first ? p.rest : r), warp_sum(fmaf(f, p.u, d * r))};
+    leader = __ffs(__ballot_sync(0xffffffffu, p.m == m)) - 1;
+    return {m, warp_sum((int)(threadIdx.x & 31) == leader ? p.rest : r), warp_sum(fmaf(f, p.u, d * r))};
+}
+__device__ __forceinline__ Part warp_join(const Part& p) {
+    int leader;
+    return warp_join(p, leader);
+}
+
+// A whole row's part, by a converged warp: whether the chunk with its maximum is worth a second look, and that look, lane i with the chunk's i-th logit (minus infinity
+// where there is none): what add_chunk has added up, in its order, goes, and the sum without the maximum comes.  (Two equal maxima are 1 and more, so there is one.)
+__device__ __forceinline__ bool few_others(const Part& p) { return p.rest < FEW_OTHERS && fabsf(p.m) < INFINITY; }
+template <int N> __device__ __forceinline__ Part others_again(const Part& p, float x) {
+    const float e = exp_of(below(x, p.m));
+    float a = 0.0f, b = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        a += __shfl_sync(0xffffffffu, e, i);
+        b += __shfl_sync(0xffffffffu, e, i + 1);
+    }
+    return {p.m, (p.rest - ((a + b) - 1.0f)) + warp_sum(x < p.m ? e : 0.0f), p.u};
 }
 
 // The joined part of the block's threads, in its first warp.  `sh` holds one Part a warp.
@@ -126,6 +155,25 @@ template <int NT> __device__ __forceinline__ Part block_join(Part p, Part* sh) {
     if (lane == 0) sh[warp] = p;
     __syncthreads();
     if (warp == 0) p = warp_join(lane < NT / 32 ? sh[lane] : Part{-INFINITY, 0.0f, 0.0f});
+    return p;
+}
+
+// The same of the parts of a row's batches (the kernel on logits), with the thread that has the maximum, and the batch that has brought it.
+struct Place { int thread, batch; };
+struct ThreadPart { Part p; Place at; };
+template <int NT> __device__ __forceinline__ Part block_join(const Run& r, int batch, ThreadPart* sh, Place& at) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int leader;
+    Part p = warp_join(r.part(), leader);
+    __syncthreads();
+    if (lane == leader) sh[warp] = {p, {(int)threadIdx.x, batch}};
+    __syncthreads();
+    if (warp == 0) {
+        ThreadPart mine = {{-INFINITY, 0.0f, 0.0f}, {0, 0}};
+        if (lane < NT / 32) mine = sh[lane];
+        p = warp_join(mine.p, leader);
+        at = {__shfl_sync(0xffffffffu, mine.at.thread, leader), __shfl_sync(0xffffffffu, mine.at.batch, leader)};
+    }
     return p;
 }
 
@@ -302,6 +350,30 @@ template <> struct Pack<__nv_bfloat16> {
     }
 };
 
+// Where the vectors of a row lie: the elements ahead of the first, and their number.
+template <typename T> struct Vectors {
+    int lead, n;
+    __device__ __forceinline__ Vectors(const T* row, int V)
+        : lead(min(V, (int)((16 - ((uintptr_t)row & 15)) % 16 / sizeof(T)))), n((V - lead) / Pack<T>::N) {}
+};
+// The i-th logit of a batch (-1: of the elements ahead of the vectors and behind them); minus infinity where there is none.  All of it is worked
+// out again: kept in registers until here it costs the loop over the row some of its own.
+template <typename T, int NT, int U> __device__ __forceinline__ float logit_at(const TokenParams& p, int r, int part, int parts, Place at, int i) {
+    constexpr int VEC = Pack<T>::N;
+    const T* row = (const T*)p.logits + (size_t)(p.rows ? p.rows[r] : r) * p.ld;
+    const Vectors<T> vecs(row, p.V);
+    int id = -1;
+    if (at.batch < 0) {
+        const int behind = vecs.lead + vecs.n * VEC + at.thread;
+        if (i == 0 && part == 0 && at.thread < vecs.lead) id = at.thread;
+        if (i == 1 && part == parts - 1 && behind < p.V) id = behind;
+    } else if (i < U * VEC) {
+        const int v = at.batch + i / VEC * NT;
+        if (v < (int)((long long)vecs.n * (part + 1) / parts)) id = vecs.lead + v * VEC + i % VEC;
+    }
+    return id >= 0 ? to_f32<T>(row[id]) : -INFINITY;
+}
+
 // A cluster of C blocks a row (C = 1: a block).  The row's 16-byte vectors are dealt to the blocks in turn ranges and, inside, to
 // the threads in batches of U: a thread's elements come by ascending id.  The few elements ahead of the first
 // 16-byte boundary and behind the last belong to the first block's first threads and the last block's first threads.
@@ -313,8 +385,8 @@ __global__ __launch_bounds__(NT, NT == 128 ? 8 : CLUSTER ? 2 : 3) void token_log
     pdl_trigger();
     constexpr int VEC = Pack<T>::N, U = 16 / VEC;
     __shared__ TopShared<NT> top;
-    __shared__ Part s_parts[32];
-    __shared__ Part s_part_of[8];                                // of the cluster's blocks, in the first one's memory
+    __shared__ ThreadPart s_parts[NT / 32];
+    __shared__ ThreadPart s_part_of[8];                          // of the cluster's blocks, in the first one's memory
     __shared__ Row s_row;
     const int tid = threadIdx.x;
     const int part = CLUSTER ? (int)cluster_rank() : 0, parts = CLUSTER ? n_parts : 1;
@@ -329,46 +401,45 @@ __global__ __launch_bounds__(NT, NT == 128 ? 8 : CLUSTER ? 2 : 3) void token_log
     const T* row = (const T*)p.logits + (size_t)(there ? at : 0) * p.ld;
     const float given = part == 0 && token >= 0 && token < V ? to_f32<T>(row[token]) : -INFINITY;
 
-    const int lead = min(V, (int)((16 - ((uintptr_t)row & 15)) % 16 / sizeof(T)));
-    const int vecs = (V - lead) / VEC, tail = lead + vecs * VEC;
+    const Vectors<T> place_of(row, V);
+    const int lead = place_of.lead, vecs = place_of.n, tail = lead + vecs * VEC;
     const int v0 = (int)((long long)vecs * part / parts) + tid, v1 = (int)((long long)vecs * (part + 1) / parts);      // this thread's first; the block's end
-    const int n_batches = v0 < v1 ? (v1 - v0 + U * NT - 1) / (U * NT) : 0;
     const Pack<T>* from = reinterpret_cast<const Pack<T>*>(row + lead);
     // the element ahead of the vectors that is this thread's, and the one behind them
     const int ahead = part == 0 && tid < lead ? tid : -1, behind = part == parts - 1 && tid < V - tail ? tail + tid : -1;
 
     Run mine;
-    float x[U * VEC];                                            // a batch
-    auto load = [&](int b) {
+    float x[U * VEC];                                            // a batch, named by its first vector
+    auto load = [&](int v) {
         Pack<T> in[U];
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int v = v0 + (b * U + i) * NT;
-            if (v < v1) in[i] = from[v];
+            if (v + i * NT < v1) in[i] = from[v + i * NT];
             else in[i].nothing();
         }
 #pragma unroll
         for (int i = 0; i < U * VEC; ++i) x[i] = in[i / VEC].at(i % VEC);
     };
-    auto id_of = [&](int b, int i) { return lead + (v0 + (b * U + i / VEC) * NT) * VEC + i % VEC; };
+    auto id_of = [&](int v, int i) { return lead + (v + i / VEC * NT) * VEC + i % VEC; };
     float second = -INFINITY;                                    // largest of the batches but the one with the maximum
-    int best_batch = -1;
+    int best = -1;                                               // that one
     const float one_ahead = ahead >= 0 ? to_f32<T>(row[ahead]) : -INFINITY, one_behind = behind >= 0 ? to_f32<T>(row[behind]) : -INFINITY;
-    for (int b = 0; b < n_batches; ++b) {
-        load(b);
+    for (int v = v0; v < v1; v += U * NT) {
+        load(v);
         const float most = most_of(x);
         if (most > mine.m) {
-            if (best_batch >= 0) second = mine.m;
-            best_batch = b;
+            if (best >= 0) second = mine.m;
+            best = v;
         } else {
             second = fmaxf(second, most);
         }
         add_chunk(mine, x, most);
     }
     const float most = mine.m;                                   // of the vectors
+    int brought = best;                                          // the batch that has brought the maximum; -1: the elements ahead of the vectors and behind them
     if (ahead >= 0 || behind >= 0) {
         const float ends[2] = {one_ahead, one_behind};
-        add_chunk(mine, ends, most_of(ends));
+        if (add_chunk(mine, ends, most_of(ends))) brought = -1;
     }
 
     if constexpr (TOP) {
@@ -380,43 +451,45 @@ __global__ __launch_bounds__(NT, NT == 128 ? 8 : CLUSTER ? 2 : 3) void token_log
             if (behind >= 0) f(key_of(one_behind, behind));
         };
         // the keys of the batch in x that can reach the bound
-        auto batch = [&](int b, u64 cut, auto f) {
+        auto batch = [&](int v, u64 cut, auto f) {
             const float least = cut_logit(cut);
 #pragma unroll
             for (int i = 0; i < U * VEC; ++i)
-                if (!(x[i] < least) && v0 + (b * U + i / VEC) * NT < v1) f(key_of(x[i], id_of(b, i)));
+                if (!(x[i] < least) && v + i / VEC * NT < v1) f(key_of(x[i], id_of(v, i)));
         };
         auto each = [&](u64 cut, auto f) {
             ends(f);
-            if (best_batch >= 0 && key_of(second, 0) < cut) {    // no other batch reaches the bound
-                load(best_batch);
-                batch(best_batch, cut, f);
+            if (best >= 0 && key_of(second, 0) < cut) {          // no other batch reaches the bound
+                load(best);
+                batch(best, cut, f);
                 return;
             }
-            for (int b = 0; b < n_batches; ++b) {
-                if (best_batch < 0 && key_of(-INFINITY, id_of(b, 0)) < cut) break;        // (equal ones go on falling with their ids)
-                load(b);
-                batch(b, cut, f);
+            for (int v = v0; v < v1; v += U * NT) {
+                if (best < 0 && key_of(-INFINITY, id_of(v, 0)) < cut) break;              // (equal ones go on falling with their ids)
+                load(v);
+                batch(v, cut, f);
             }
         };
         // The largest of the vectors lies somewhere in its batch: from the first to the last id of it, unless there is nothing but minus infinity.
         u64 low = end_best, high = end_best;
-        if (n_batches > 0) {
-            const int b = max(best_batch, 0);
-            high = max(high, key_of(most, id_of(b, 0)));
-            low = max(low, key_of(most, best_batch < 0 ? id_of(b, 0) : id_of(b, U * VEC - 1)));
+        const int likely = best < 0 ? v0 : best;
+        if (v0 < v1) {
+            high = max(high, key_of(most, id_of(likely, 0)));
+            low = max(low, key_of(most, best < 0 ? id_of(v0, 0) : id_of(best, U * VEC - 1)));
         }
         if (!select_top<NT, VEC>(top, low, high, p.k, each)) {
             // many equal ones: with the places of the maxima, the first ids are told from the others
-            u64 best = end_best;
-            if (n_batches > 0) {
-                load(max(best_batch, 0));
-                batch(max(best_batch, 0), key_of(most, 0x7fffffff), [&](u64 key) { best = max(best, key); });
+            u64 key_best = end_best;
+            if (v0 < v1) {
+                load(likely);
+                batch(likely, key_of(most, 0x7fffffff), [&](u64 key) { key_best = max(key_best, key); });
             }
-            if (!select_top<NT, VEC>(top, best, best, p.k, each)) one_by_one<NT>(top, p.k, each);
+            if (!select_top<NT, VEC>(top, key_best, key_best, p.k, each)) one_by_one<NT>(top, p.k, each);
         }
     }
-    Part all = block_join<NT>(mine.part(), s_parts);
+    Place place;
+    Part all = block_join<NT>(mine, brought, s_parts, place);
+    int owner = part;                                            // the block with the maximum
     if (CLUSTER) {
         // every block stores its part and its list into the first one's memory, and all but that one may leave
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");         // every block runs: its memory may be written
@@ -425,6 +498,8 @@ __global__ __launch_bounds__(NT, NT == 128 ? 8 : CLUSTER ? 2 : 3) void token_log
             asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(all.m) : "memory");
             asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(all.rest) : "memory");
             asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(all.u) : "memory");
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + 12), "r"(place.thread) : "memory");
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + 16), "r"(place.batch) : "memory");
         }
         if constexpr (TOP) {
             const uint32_t to = map_to_cta((uint32_t)__cvta_generic_to_shared(top.joined) + 8u * (uint32_t)(part * p.k), 0);
@@ -432,8 +507,12 @@ __global__ __launch_bounds__(NT, NT == 128 ? 8 : CLUSTER ? 2 : 3) void token_log
         }
         cluster_sync_all();
         if (part != 0) return;
-        if (tid < 32) all = warp_join(tid < parts ? s_part_of[tid] : Part{-INFINITY, 0.0f, 0.0f});
+        if (tid < 32) {
+            all = warp_join(tid < parts ? s_part_of[tid].p : Part{-INFINITY, 0.0f, 0.0f}, owner);
+            place = s_part_of[owner].at;
+        }
     }
+    if (tid < 32 && few_others(all)) all = others_again<U * VEC>(all, logit_at<T, NT, U>(p, r, owner, parts, place, tid));
     if (tid == 0) {
         const Row w = row_of(all);
         s_row = w;
@@ -530,7 +609,7 @@ struct HeadParams {
     const int32_t* tokens;
     float scale, cap;
     int k;
-    float* stats;                                                  // [3][2 splits][n]: m, s - 1, u
+    float* stats;                                                  // [3][2 splits][n]: a part's m, s - 1, u
     float* given;                                                  // [n] logits of the given tokens
     u64* keys;                                                     // [n][2 splits][k]
     int* err;
@@ -835,9 +914,10 @@ __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
             if (row_on) {
                 const int parts = 2 * p.splits, part = 2 * (u / p.row_blocks) + half;
                 float* to = p.stats + (size_t)part * p.n + row;
-                to[0] = mine.m;
-                to[(size_t)parts * p.n] = mine.part().rest;
-                to[(size_t)2 * parts * p.n] = mine.u;
+                const Part all = mine.part();
+                to[0] = all.m;
+                to[(size_t)parts * p.n] = all.rest;
+                to[(size_t)2 * parts * p.n] = all.u;
                 if constexpr (TOP > 0) {
                     u64* keys = p.keys + ((size_t)row * parts + part) * p.k;
 #pragma unroll

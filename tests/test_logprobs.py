@@ -559,3 +559,66 @@ def test_head_refusals(monkeypatch):
     for cap in (0.0, -1.0, 1e-50, 1e39, float("nan")):
         refused("positive", soft_cap=cap)
     refused("dtype", hidden=_Fake(4, 64, dtype=torch.float16), weight=_Fake(100, 64, dtype=torch.float16))
+
+
+# ---------------------------------------------------------------- nearly all of a row's probability on one token
+APART = (14.0, 16.125, 18.25)          # exact in bfloat16: the second token has 8e-7, 1e-7 and 1.2e-8
+# The leading logit is 0, so differences are exact.  exp(-d): d * log2(e) is rounded twice, each time by 2^-24 of up to 18.25 in natural units, and the
+# exponential is off by 2^-22 of itself: 2.4e-6 in all; a handful of roundings of the sums, log1p and the quotient are 4e-7.
+PEAKED = 3e-6
+
+
+def near_relatively(got, want, also=0.0):
+    assert bool(((got.double() - want).abs() <= PEAKED * want.abs() + also).all()), (got, want)
+
+
+def check_peaked(got, apart, leads, also=0.0):
+    """Rows whose only logits are 0 and -apart; ``leads``: which rows ask for the leading token; ``also``: an absolute error that is allowed besides."""
+    d = torch.tensor(apart, dtype=torch.float64)
+    e = torch.exp(-d)
+    rest = torch.log1p(e)
+    near_relatively(got[0], torch.where(leads, -rest, -d - rest), also)
+    near_relatively(got[1], rest + d * e / (1 + e), also)
+    near_relatively(got[2], rest, also)
+    near_relatively(got[4], torch.stack((-rest, -d - rest), 1), also if isinstance(also, float) else also[:, None])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,repeats", [(300, 1), (20000, 1), (20000, 3), (151936, 1)])
+def test_tokens_peaked_rows_in_any_order(V, repeats, dtype):
+    """The leading token before and behind the second one: in one batch of a thread, in a later one, in another thread or block."""
+    places = [p for p in (1, 2, 70, 2049, 8193, V - 1) if p < V]
+    rows = [(a, b, d) for a in places for b in places if a != b for d in APART] * repeats
+    x = torch.full((len(rows), V), -math.inf)
+    for r, (a, b, d) in enumerate(rows):
+        x[r, a], x[r, b] = 0.0, -d
+    leads = torch.arange(len(rows)) % 2 == 0
+    t = torch.tensor([a if r % 2 == 0 else b for r, (a, b, d) in enumerate(rows)], dtype=torch.int32, device=DEV)
+    got = call(x.to(dtype).to(DEV), t, 2)
+    check_peaked(got, [d for _, _, d in rows], leads)
+    assert got[3].tolist() == [[a, b] for a, b, _ in rows]
+    for g, w in zip(call(x.to(dtype).to(DEV), t, 0)[:3], got[:3]):
+        near_relatively(g, w.double())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [5, 40, 100, 300])
+def test_head_peaked_rows_in_any_order(n):
+    """The same from hidden states, every row one column of the weights: in the 32 ids a thread takes at a time, in later ones, in another tile or range.  Among the
+    32 that hold the leading one the others are rounded to 2^-24 of its 1 (twice at most) where the logits are never written."""
+    V = 20000
+    pairs = [(1, 2), (2, 1), (1, 70), (70, 1), (1, 40), (40, 1), (1, 300), (300, 1), (3, 19990), (19990, 3), (64, 129), (129, 64)]
+    w = torch.full((V, 64), -2000.0)
+    apart = [APART[j % 3] for j in range(len(pairs))]
+    for j, (a, b) in enumerate(pairs):
+        w[a, j], w[b, j] = 0.0, -apart[j]
+    at = [r % len(pairs) for r in range(n)]
+    h = torch.zeros(n, 64)
+    h[torch.arange(n), at] = 1.0
+    leads = torch.arange(n) % 2 == 0
+    t = torch.tensor([pairs[j][r % 2] for r, j in enumerate(at)], dtype=torch.int32, device=DEV)
+    got = head(h.to(torch.bfloat16).to(DEV), w.to(torch.bfloat16).to(DEV), t, 2)
+    together = torch.tensor([pairs[j][0] // 32 == pairs[j][1] // 32 and n > 32 for j in at])
+    check_peaked(got, [apart[j] for j in at], leads, together * 2.0 ** -23)
+    assert got[3].tolist() == [list(pairs[j]) for j in at]
