@@ -353,7 +353,8 @@ class Engine:
         cands = self._candidates_to_host(logits, cand_rows, n_cand) if cand_rows else None
         rows_host = self._rows_to_host(logits, host_rows) if host_rows else None
         prob_rows = [i for i, r in enumerate(reqs) if r.params.logprobs is not None and i not in set(host_rows)]
-        probs = self._probs_to_host(logits, prob_rows, max(reqs[i].params.logprobs for i in prob_rows)) if prob_rows else None
+        # (one alternative at least where the host draws: the row's maximum is what the drawn logit is told from)
+        probs = self._probs_to_host(logits, prob_rows, max([reqs[i].params.logprobs for i in prob_rows] + [1] * bool(cand_rows))) if prob_rows else None
         if look_ahead and not host_rows and self._ahead is None:
             self._prepare_ahead(reqs)                      # the GPU is busy: plan and lay out the next step meanwhile
         torch.cuda.current_stream().synchronize()
@@ -383,15 +384,17 @@ class Engine:
                 for j, tok in zip(sure, sample_candidates([self._drawer(r) for r in rq], ids[sure], vals[sure], windows)):
                     out[cand_rows[j]] = tok
         if prob_rows:
-            logprob, lse, top_ids, top_logprobs = probs
+            logprob, top_ids, top_logprobs = probs
             place = {i: j for j, i in enumerate(cand_rows)}
             for q, i in enumerate(prob_rows):
                 value, j = logprob[q], place.get(i)
                 if j is not None:                          # the host has picked: one of the candidates, whose logits are here
                     if cands[2][j] or self._distrust_candidates:
                         continue
+                    # (x - m) + the maximum's own log probability, as the kernel rounds it: the value that an alternative of this id has
+                    vals = cands[1][j]
                     at = np.nonzero(cands[0][j] == out[i])[0]
-                    value = np.float32(cands[1][j][at[0]] - lse[q]) if at.size else -np.inf
+                    value = (vals[at[0]] - vals[0]) + top_logprobs[q, 0] if at.size and vals[at[0]] > -np.inf else -np.inf
                 n_top = min(reqs[i].params.logprobs, top_ids.shape[1])
                 reqs[i].sampler.probs.append(TokenProbs(out[i], float(value), [(int(a), float(b)) for a, b in zip(top_ids[q, :n_top],
                                                                                                                   top_logprobs[q, :n_top])]))
@@ -407,11 +410,11 @@ class Engine:
         return drawer if told else r.sampler
 
     def _probs_to_host(self, logits: torch.Tensor, rows: List[int], top: int):
-        """Of each of ``rows``: the log probability of the token that the device has picked, ln sum exp of the raw logits and the ``top`` likeliest tokens,
-        copied to pinned memory (queued; the caller synchronises the stream): logprob, lse, ids, log probabilities as numpy views."""
+        """Of each of ``rows``: the log probability of the token that the device has picked and the ``top`` likeliest tokens, copied to pinned
+        memory (queued; the caller synchronises the stream): logprob, ids, log probabilities as numpy views."""
         n, cap, top = len(rows), self.runner.R_max, min(top, logits.shape[1])
         if self._prob_bufs is None or self._prob_bufs[4] < top:
-            words = cap * (2 + 2 * top)
+            words = cap * (1 + 2 * top)
             self._prob_bufs = (torch.empty(cap, dtype=torch.int32, pin_memory=True), torch.empty((2, cap), dtype=torch.int32, device=self.device),
                                torch.empty(words, dtype=torch.float32, device=self.device), torch.empty(words, dtype=torch.float32, pin_memory=True), top)
         idx_host, idx_dev, dev, host, _ = self._prob_bufs
@@ -419,12 +422,12 @@ class Engine:
         idx, tokens = idx_dev[0, :n], idx_dev[1, :n]
         idx.copy_(idx_host[:n], non_blocking=True)
         ops.gather_rows(self._picked_dev.view(-1, 1), idx, tokens.view(-1, 1))
-        ends = [n, 2 * n, (2 + top) * n, (2 + 2 * top) * n]
-        ids = dev[ends[1]:ends[2]].view(torch.int32).view(n, top) if top else None
-        ops.token_logprobs(logits, tokens, dev[:n], lse=dev[n:ends[1]], top_ids=ids, top_logprobs=dev[ends[2]:ends[3]].view(n, top) if top else None, rows=idx)
-        host[:ends[3]].copy_(dev[:ends[3]], non_blocking=True)
+        ends = [n, (1 + top) * n, (1 + 2 * top) * n]
+        ids = dev[n:ends[1]].view(torch.int32).view(n, top) if top else None
+        ops.token_logprobs(logits, tokens, dev[:n], top_ids=ids, top_logprobs=dev[ends[1]:ends[2]].view(n, top) if top else None, rows=idx)
+        host[:ends[2]].copy_(dev[:ends[2]], non_blocking=True)
         h = host.numpy()
-        return h[:n], h[n:ends[1]], h[ends[1]:ends[2]].view(np.int32).reshape(n, top), h[ends[2]:ends[3]].reshape(n, top)
+        return h[:n], h[n:ends[1]].view(np.int32).reshape(n, top), h[ends[1]:ends[2]].reshape(n, top)
 
     def _candidates_to_host(self, logits: torch.Tensor, rows: List[int], n_cand: int):
         """The ``n_cand`` largest logits of each of ``rows`` with their ids, found by the engine's own kernel and

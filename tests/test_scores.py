@@ -227,3 +227,27 @@ def test_a_head_of_its_own_is_scored_from_its_logits(folders):
     a, b = got
     assert float((a.logprob - b.logprob).abs().max()) < TOL and float((a.entropy - b.entropy).abs().max()) < TOL
     assert float((a.top_logprobs - b.top_logprobs).abs().max()) < TOL
+
+
+def test_a_drawn_token_has_the_value_of_its_entry_among_the_alternatives(folders):
+    """A token that the host draws from its candidates, or the device picks, and that is among the alternatives too has one value, bit for bit; one that is not, and a
+    draw without alternatives, the value that the same draw has where it is listed."""
+    from airun_b200 import SamplingParams as S
+    draws = [dict(S(seed=3).__dict__), dict(S(seed=5, temperature=0.7, top_p=0.9, repeat_penalty=1.0).__dict__), dict(S(seed=11, temperature=3.0, top_k=60).__dict__),
+             dict(S.greedy().__dict__), dict(S(temperature=0.0, repeat_penalty=1.3).__dict__)]
+    eng = engine(folders, "D", max_batch_tokens=64, max_requests=8)
+    prompts = [random_tokens(5 + 7 * i, eng.config.vocab_size, 80 + i) for i in range(len(draws))]
+    results = {}
+    for told in (0, 1, 100):
+        results[told] = eng.generate(prompts, [S(**dict(p, logprobs=told)) for p in draws], max_new_tokens=12)
+    listed = 0
+    for few, one, many in zip(results[0], results[1], results[100]):
+        assert few.token_ids == one.token_ids == many.token_ids
+        for a, b, c in zip(few.logprobs, one.logprobs, many.logprobs):
+            assert a.top == [] and len(b.top) == 1 and len(c.top) == 100 and b.top[0] == c.top[0]
+            assert a.logprob == b.logprob == c.logprob
+            entry = dict(c.top).get(c.token)
+            if entry is not None:
+                listed += 1
+                assert c.logprob == entry
+    assert listed > 30
