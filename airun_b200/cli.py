@@ -265,6 +265,26 @@ def cmd_bench(a) -> int:
     return 0
 
 
+LOSS_BLOCK = 1 << 25                   # logits that are held in 64 bits at a time: 256 MiB
+
+
+def place_losses(logits, targets):
+    """The losses (nats) of ``targets`` under softmax of the rows of ``logits`` [n, V], and whether each is the row's largest: in 64 bits, on the logits' device, a block
+    of rows at a time.  A row with a logit that is not a number has no loss (NaN), unlike in Engine.score, where such a logit counts as minus infinity: a
+    measure of a model says so where the model is broken."""
+    import torch
+    n, V = logits.shape
+    want = torch.as_tensor(targets, dtype=torch.long).to(logits.device)
+    losses, best = [], []
+    step = max(1, LOSS_BLOCK // V)
+    for at in range(0, n, step):
+        t = want[at:at + step]
+        rows = logits[at:at + step]
+        losses += (-torch.log_softmax(rows.double(), dim=-1).gather(1, t[:, None])[:, 0]).tolist()
+        best += (rows.argmax(dim=-1) == t).tolist()
+    return losses, best
+
+
 def cmd_perplexity(a) -> int:
     """Scores a file of token ids as the reference's ``airun perplexity`` scores a text
     (crates/airun-cli/src/perplexity.rs:97-222): one pass over everything, token by token, or with
@@ -272,10 +292,7 @@ def cmd_perplexity(a) -> int:
     predictions of their second half; ``--batched`` feeds a pass in one step (the kernels of prompt
     portions) instead of one token at a time (the decode kernels).  The two agree to rounding."""
     import math
-    import torch
     from . import Engine, EngineOptions, StepEntry
-    from .kernels import ops
-    from .parts.base import TokenScores
     if not a.file:
         raise SystemExit("perplexity needs --file with the token ids to score (the engine has no tokenizer)")
     with open(a.file) as f:
@@ -297,37 +314,36 @@ def cmd_perplexity(a) -> int:
     eng = Engine.from_folder(a.model, EngineOptions(dtype=a.dtype, cache_tokens=longest + 64, max_requests=1,
                                                      max_batch_tokens=max(longest if a.batched else 1, 16),
                                                      max_context=longest + 64))
+    V = eng.config.vocab_size
+    bad = [t for t in ids[:passes[-1][1]] if not 0 <= t < V]
+    if bad:
+        raise SystemExit(f"the file holds token ids outside [0, {V}): {bad[:5]}")
     losses = []                                    # (position, token, loss)
     total, top1 = 0.0, 0
 
-    def note(scores, first):
-        """Scores of the tokens at the places from ``first`` on; their log probabilities are worked out on the GPU."""
+    def note(logits, first):
+        """The rows of ``logits`` tell the tokens at the places from ``first`` on."""
         nonlocal total, top1
-        for k, (lp, best) in enumerate(zip(scores.logprob.tolist(), scores.top_ids[:, 0].tolist())):
-            pos = first + k
-            top1 += int(best == ids[pos])
-            total -= lp
-            losses.append((pos, ids[pos], -lp))
-
-    one = TokenScores.empty(1, 1, eng.device)
-    target = torch.zeros(1, dtype=torch.int32, device=eng.device)
+        places = range(first, first + logits.shape[0])
+        for pos, loss, best in zip(places, *place_losses(logits, [ids[pos] for pos in places])):
+            top1 += int(best)
+            total += loss
+            losses.append((pos, ids[pos], loss))
 
     for start, end, first in passes:
         slot = eng.manager.add_request("t").slot   # an empty context for every pass
         eng.storage.zero_state_slot(slot)
         if a.batched:
             rows = [r for r in range(end - start) if r >= first and r + 1 < end - start]
-            scores = eng.runner.score([StepEntry("t", ids[start:end], tuple(rows))], [ids[start + r + 1] for r in rows], top=1)
-            if scores is not None:
-                note(scores, start + rows[0] + 1)
+            logits = eng.runner.step([StepEntry("t", ids[start:end], tuple(rows))])
+            if logits is not None:
+                note(logits, start + rows[0] + 1)
         else:
             for i in range(start, end - 1):
                 wanted = i - start >= first
                 logits = eng.runner.step([StepEntry("t", [ids[i]], (0,) if wanted else ())])
                 if wanted:
-                    target.fill_(ids[i + 1])
-                    ops.token_logprobs(logits, target, one.logprob, one.entropy, None, one.top_ids, one.top_logprobs)
-                    note(one, i + 1)
+                    note(logits, i + 1)
         eng.manager.free_request("t")
         if len(passes) > 1:
             print(f"[{len(losses) // max(end - start - 1 - first, 1)}]{math.exp(total / max(len(losses), 1)):.4f},",
@@ -339,9 +355,12 @@ def cmd_perplexity(a) -> int:
     mean = total / n
     print(f"\n{n} tokens scored\n  mean loss   {mean:.4f} nats/token\n  perplexity  {math.exp(mean):.2f}\n"
           f"  top-1       {100.0 * top1 / n:.1f}% ({top1}/{n})")
+    broken = sum(not math.isfinite(loss) for _, _, loss in losses)
+    if broken:
+        print(f"  not finite  the losses of {broken} of the {n} tokens")
     if a.worst > 0:
         print("\nworst-predicted tokens:")
-        for pos, tok, nll in sorted(losses, key=lambda t: -t[2])[:a.worst]:
+        for pos, tok, nll in sorted(losses, key=lambda t: -math.inf if math.isnan(t[2]) else -t[2])[:a.worst]:
             print(f"  pos {pos:>4}  loss {nll:>8.3f}  token {tok}")
     return 0
 

@@ -474,7 +474,7 @@ class Engine:
     def score(self, prompts: Union[Sequence[int], Sequence[Sequence[int]]], top: int = 0) -> Union[PromptScore, List[PromptScore]]:
         """Log probabilities of the prompts' own tokens, with the entropies they come from and the ``top`` likeliest tokens at every place, without
         generating anything: for one prompt (a list of ids) or several, which share steps of up to ``max_batch_tokens``.  The logits are
-        not kept (Head.score).  Between requests only: raises RuntimeError while any is running or waiting."""
+        not kept (Head.score); one that is not a number counts as minus infinity.  Between requests only: raises RuntimeError while any is running or waiting."""
         single = len(prompts) > 0 and not isinstance(prompts[0], (list, tuple, np.ndarray))
         plist = [[int(t) for t in p] for p in ([prompts] if single else prompts)]
         V = self.config.vocab_size

@@ -622,3 +622,27 @@ def test_head_peaked_rows_in_any_order(n):
     together = torch.tensor([pairs[j][0] // 32 == pairs[j][1] // 32 and n > 32 for j in at])
     check_peaked(got, [apart[j] for j in at], leads, together * 2.0 ** -23)
     assert got[3].tolist() == [list(pairs[j]) for j in at]
+
+
+# ---------------------------------------------------------------- the command that measures a model
+def test_losses_of_places_are_worked_out_in_64_bits(monkeypatch):
+    """To the last digits of 64 bits (a sum of 5,000 terms: 1e-13), in blocks of rows too; a logit that is not a number leaves its row without a loss."""
+    from airun_b200 import cli
+    g = torch.Generator().manual_seed(2)
+    x = 5 * torch.randn(40, 5000, generator=g)
+    x[3, 17] += 60.0                                   # one leading token: a loss of about 1e-20
+    t = torch.randint(0, 5000, (40,), generator=g)
+    t[3], t[4] = 17, int(x[4].argmax())
+    losses, best = cli.place_losses(x, t.tolist())
+    d = x.numpy().astype(np.longdouble) - x.numpy().max(1, keepdims=True).astype(np.longdouble)
+    want = np.log(np.exp(d).sum(1)) - d[np.arange(40), t.numpy()]
+    assert np.abs(np.array(losses) - want.astype(np.float64)).max() <= 1e-12
+    assert best == [bool(x[i].argmax() == t[i]) for i in range(40)] and best[3] and best[4]
+    x[5, 9] = math.nan
+    x[6] = math.nan
+    x[7, int(t[7])] = -math.inf
+    losses, _ = cli.place_losses(x, t.tolist())
+    assert math.isnan(losses[5]) and math.isnan(losses[6]) and losses[7] == math.inf and all(math.isfinite(v) for v in losses[:5] + losses[8:])
+    monkeypatch.setattr(cli, "LOSS_BLOCK", 10001)      # two rows a block
+    again, best_again = cli.place_losses(x, t.tolist())
+    assert np.array_equal(again, losses, equal_nan=True) and best_again[:5] == best[:5]

@@ -251,3 +251,34 @@ def test_a_drawn_token_has_the_value_of_its_entry_among_the_alternatives(folders
                 listed += 1
                 assert c.logprob == entry
     assert listed > 30
+
+
+@pytest.mark.parametrize("batched", [[], ["--chunk", "20", "--batched"]])
+def test_perplexity_shows_a_broken_model_and_refuses_ids_it_does_not_have(batched, folders, tmp_path, monkeypatch, capsys):
+    """One logit that is not a number is a loss that is not one, and so is the mean; a last id behind the vocabulary ends the command."""
+    import airun_b200
+    from airun_b200.cli import main
+    V = engine(folders, "B").config.vocab_size
+    f = tmp_path / "ids.txt"
+    f.write_text(" ".join(map(str, random_tokens(40, V, 8))))
+    args = ["perplexity", folders["B"], "-f", str(f), "--dtype", "float32"] + batched
+    assert main(args) == 0
+    sound = capsys.readouterr().out
+    assert "not finite" not in sound and "nan" not in sound
+    load = airun_b200.Engine.from_folder
+
+    def broken(*a, **k):
+        eng = load(*a, **k)
+        eng.model.head.weight = eng.model.head.weight.clone()
+        eng.model.head.weight[7, 3] = math.nan
+        return eng
+
+    monkeypatch.setattr(airun_b200.Engine, "from_folder", broken)
+    assert main(args + ["--worst", "1"]) == 0
+    out = capsys.readouterr().out
+    n = 18 if batched else 39
+    assert "mean loss   nan" in out and f"the losses of {n} of the {n} tokens" in out
+    monkeypatch.setattr(airun_b200.Engine, "from_folder", load)
+    f.write_text(f.read_text() + f" {V}")
+    with pytest.raises(SystemExit, match="outside"):
+        main(["perplexity", folders["B"], "-f", str(f), "--dtype", "float32"])
