@@ -203,18 +203,24 @@ class TokenScores:
 
 
 class Head(Part):
-    """forward(ctx, h [rows, hidden] in the compute type, out float32 [rows, vocab]).
-    score(ctx, h, tokens int32 [rows], scores): log probabilities of the tokens under the rows' distributions; a head that can tell them
-    without the rows' logits has its own."""
+    """forward(ctx, h [rows, hidden] in the compute type, out float32 [rows, vocab]); ``V``: the vocabulary's size.
+    score(ctx, h, tokens int32 [rows], scores): log probabilities of the tokens under the rows' distributions, from the logits of a block of rows at a
+    time; a head that can tell them without the rows' logits has its own."""
+
+    V: int
 
     def forward(self, ctx, h: torch.Tensor, out: torch.Tensor) -> None:
         raise NotImplementedError
 
     def score(self, ctx, h: torch.Tensor, tokens: torch.Tensor, scores: TokenScores) -> None:
         from ..kernels import ops
-        logits = ctx.ws_main.alloc((h.shape[0], self.V), torch.float32)
-        self.forward(ctx, h, logits)
-        ops.token_logprobs(logits, tokens, scores.logprob, scores.entropy, None, scores.top_ids, scores.top_logprobs)
+        n, step = h.shape[0], max(1, ops.HEAD_CHUNK // self.V)
+        logits = ctx.ws_main.alloc((min(n, step), self.V), torch.float32)
+        part = lambda t, a: None if t is None else t[a:a + step]      # noqa: E731
+        for a in range(0, n, step):
+            x = logits[:min(step, n - a)]
+            self.forward(ctx, h[a:a + step], x)
+            ops.token_logprobs(x, part(tokens, a), part(scores.logprob, a), part(scores.entropy, a), None, part(scores.top_ids, a), part(scores.top_logprobs, a))
 
 
 class ResidualInput(Part):

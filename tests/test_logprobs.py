@@ -646,3 +646,40 @@ def test_losses_of_places_are_worked_out_in_64_bits(monkeypatch):
     monkeypatch.setattr(cli, "LOSS_BLOCK", 10001)      # two rows a block
     again, best_again = cli.place_losses(x, t.tolist())
     assert np.array_equal(again, losses, equal_nan=True) and best_again[:5] == best[:5]
+
+
+def test_a_head_that_only_forms_logits_is_scored_in_blocks_of_rows(monkeypatch):
+    """Head.score holds no more than HEAD_CHUNK logits, however many rows there are; every row meets its own token and place."""
+    from types import SimpleNamespace
+    from airun_b200.engine.batch import Workspace
+    from airun_b200.kernels import ops
+    from airun_b200.parts.base import Head, TokenScores
+    g = torch.Generator().manual_seed(1)
+    w = torch.randn(50, 8, generator=g)
+
+    class Plain(Head):
+        V = 50
+
+        def forward(self, ctx, h, out):
+            out.copy_(h @ w.t())
+
+    def told(logits, tokens, logprob, entropy, lse, top_ids, top_logprobs):
+        held.append(logits.numel())
+        lp, H, _, ids, tops = plain(logits.double(), tokens, 3)
+        for place, value in ((logprob, lp), (entropy, H), (top_ids, ids), (top_logprobs, tops)):
+            if place is not None:
+                place.copy_(value)
+
+    monkeypatch.setattr(ops, "token_logprobs", told)
+    for chunk, most in ((1 << 26, 23), (350, 7), (49, 1)):
+        monkeypatch.setattr(ops, "HEAD_CHUNK", chunk)
+        for top in (0, 3):
+            held, h, t = [], torch.randn(23, 8, generator=g), torch.randint(0, 50, (23,), generator=g, dtype=torch.int32)
+            ctx, scores = SimpleNamespace(ws_main=Workspace(torch.device("cpu"), 1 << 10)), TokenScores.empty(23, top, "cpu")
+            Plain().score(ctx, h, t, scores)
+            want = plain((h @ w.t()).double(), t, 3)
+            near(scores.logprob, want[0]), near(scores.entropy, want[1])
+            assert max(held) == most * 50 and sum(held) == 23 * 50 and ctx.ws_main.bytes() <= max(1 << 10, 4 * 50 * most + 256)
+            if top:
+                assert torch.equal(scores.top_ids.long(), want[3])
+                near(scores.top_logprobs, want[4])
