@@ -25,7 +25,7 @@ _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16}
 
 DEV_ERR_BITS = {1: "a block-table entry outside the page pool", 2: "a token naming a request outside the batch",
                 4: "a token id outside the vocabulary", 8: "a bounded device-side wait ran out",
-                16: "a row of an expert or a segment of a prompt outside its buffer"}
+                16: "a row of logits or of an expert, or a segment of a prompt, outside its buffer"}
 
 
 class KernelError(RuntimeError):

@@ -683,3 +683,8 @@ def test_a_head_that_only_forms_logits_is_scored_in_blocks_of_rows(monkeypatch):
             if top:
                 assert torch.equal(scores.top_ids.long(), want[3])
                 near(scores.top_logprobs, want[4])
+
+
+def test_a_bad_row_is_described_as_one_of_logits_too():
+    from airun_b200.kernels import ops
+    assert "row of logits" in ops.describe_device_error(16) and "expert" in ops.describe_device_error(16) and "segment" in ops.describe_device_error(16)
