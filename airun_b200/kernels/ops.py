@@ -1281,6 +1281,7 @@ def largest_logits(logits: torch.Tensor, rows: torch.Tensor, n: int, n_cand: int
 
 
 TOP_LOGPROBS_MAX = 128
+LOGITS_MAX, LOGPROB_ROWS_MAX = 0x7fff0000, 1 << 27        # rows or columns of logits, tokens of a call: what the kernels' 32-bit numbers of them hold
 
 
 def _logprob_outputs(n: int, vocab: int, tokens, logprob, entropy, lse, top_ids, top_logprobs) -> int:
@@ -1323,11 +1324,15 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Te
     if len(shape) != 2 or shape[1] == 0 or logits.stride(1) != 1:
         raise KernelError("logits must be row-major [rows, V]")
     R, V = shape
+    if R > LOGITS_MAX or V > LOGITS_MAX or n > LOGPROB_ROWS_MAX:
+        raise KernelError(f"logits of at most {LOGITS_MAX} rows and columns, for at most {LOGPROB_ROWS_MAX} tokens")
     k = _logprob_outputs(n, V, tokens, logprob, entropy, lse, top_ids, top_logprobs)
     if rows is None:
         _need(R >= n, "a row of logits for every token")
     else:
         _need(rows.dtype == torch.int32 and rows.shape == (n,) and rows.is_contiguous() and (R > 0 or n == 0), "rows must be int32 [n], of one row of logits or more")
+    if err is not None:
+        _need(err.dtype == torch.int32 and err.numel() == 1, "err must be one int32")
     ld = logits.stride(0) if R > 1 else V
     _need(ld >= V, "rows of logits must not overlap")
     f = _fn("logprobs", "airun_token_logprobs", _TOKEN_LOGPROBS)
@@ -1360,6 +1365,7 @@ def head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tens
     _dt(hidden)
     _need(hidden.stride(1) == 1 and weight.stride(1) == 1, "hidden and weight must be row-major")
     n, V = hs[0], wsh[0]
+    _need(max(V, hs[1]) <= LOGITS_MAX and n <= LOGPROB_ROWS_MAX, f"at most {LOGPROB_ROWS_MAX} rows, and {LOGITS_MAX} tokens and values")
     _need((n <= 1 or hidden.stride(0) >= hs[1]) and (V <= 1 or weight.stride(0) >= hs[1]), "rows of hidden and weight must not overlap")
     _need(tokens.dim() == 1 and tokens.shape[0] == n, "a token for every row")
     _logprob_outputs(n, V, tokens, logprob, entropy, lse, top_ids, top_logprobs)

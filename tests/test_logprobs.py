@@ -688,3 +688,33 @@ def test_a_head_that_only_forms_logits_is_scored_in_blocks_of_rows(monkeypatch):
 def test_a_bad_row_is_described_as_one_of_logits_too():
     from airun_b200.kernels import ops
     assert "row of logits" in ops.describe_device_error(16) and "expert" in ops.describe_device_error(16) and "segment" in ops.describe_device_error(16)
+
+
+class _Huge:
+    """The same as _Fake without memory: sizes that only the checks see."""
+
+    def __new__(cls, *shape, dtype=torch.float32):
+        class OnGpu(torch.Tensor):
+            is_cuda = True
+        return torch.empty(*shape, dtype=dtype, device="meta").as_subclass(OnGpu)
+
+
+def test_refusals_of_sizes_beyond_32_bits_and_of_other_error_words(monkeypatch):
+    """Numbers of rows, columns and tokens go to the kernels in 32 bits: what they would lose is refused, not cut off.  The device writes an int32 where the error word is."""
+    from airun_b200.kernels import ops
+    monkeypatch.setattr(ops, "_fn", lambda *a, **k: pytest.fail("launched"))
+    monkeypatch.setattr(ops, "_here", ops._cuda)
+    t, lp = _Fake(4, dtype=torch.int32), _Fake(4)
+    for R, V in (((1 << 32) + 4, 10), (1 << 31, 1), (4, (1 << 32) + 10), (4, 1 << 31)):
+        with pytest.raises(ops.KernelError, match="at most"):
+            ops.token_logprobs(_Huge(R, V), t, lp)
+    n = (1 << 32) + 2
+    with pytest.raises(ops.KernelError, match="at most"):
+        ops.token_logprobs(_Huge(4, 10), _Huge(n, dtype=torch.int32), _Huge(n), rows=_Huge(n, dtype=torch.int32))
+    err = _Fake(1, dtype=torch.int32)
+    for n, V, H in ((4, (1 << 32) + 16, 8), (4, 16, (1 << 32) + 8), ((1 << 32) + 1, 16, 8)):
+        with pytest.raises(ops.KernelError, match="at most"):
+            ops.head_logprobs(_Huge(n, H, dtype=torch.bfloat16), _Huge(V, H, dtype=torch.bfloat16), _Huge(n, dtype=torch.int32), _Huge(n), err)
+    for bad in (_Fake(1), _Fake(1, dtype=torch.int64), _Fake(2, dtype=torch.int32), _Fake(0, dtype=torch.int32)):
+        with pytest.raises(ops.KernelError, match="one int32"):
+            ops.token_logprobs(_Fake(4, 100), t, lp, err=bad)
