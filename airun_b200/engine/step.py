@@ -219,12 +219,13 @@ class StepRunner:
             raise StepError(f"{len(targets)} targets for {n} wanted places")
         if not 0 <= top <= min(ops.TOP_LOGPROBS_MAX, self.model.V):
             raise StepError(f"{top} alternatives a place, at most {min(ops.TOP_LOGPROBS_MAX, self.model.V)} can be told")
+        asked = np.fromiter((t if 0 <= t < self.model.V else -1 for t in targets), dtype=np.int32, count=n)
         self.reserve(entries)
         ctx, n_want = self.build_context(entries)
         scores = None
         if n:
             scores = TokenScores.empty(n, top, self.device)
-            tokens = torch.as_tensor(np.asarray(targets, dtype=np.int32)).to(self.device)
+            tokens = torch.as_tensor(asked).to(self.device)
             self.model.forward(ctx, self._view("want_rows"), n_want, score=(tokens, scores))
         else:
             self.model.forward(ctx, None, 0)

@@ -282,3 +282,16 @@ def test_perplexity_shows_a_broken_model_and_refuses_ids_it_does_not_have(batche
     f.write_text(f.read_text() + f" {V}")
     with pytest.raises(SystemExit, match="outside"):
         main(["perplexity", folders["B"], "-f", str(f), "--dtype", "float32"])
+
+
+def test_targets_far_outside_the_vocabulary_ask_for_none(folders):
+    """Ids that 32 bits do not hold are ids outside the vocabulary like any other."""
+    from airun_b200 import StepEntry
+    eng = engine(folders, "A")
+    V = eng.config.vocab_size
+    eng.manager.add_request("a")
+    got = eng.runner.score([StepEntry("a", [1, 2, 3, 4, 5, 6], range(6))], [2, 1 << 40, -1 << 40, V, (1 << 32) + 2, np.int64(3)])
+    lp = got.logprob.tolist()
+    assert lp[1:5] == [-math.inf] * 4 and math.isfinite(lp[0]) and math.isfinite(lp[5])
+    eng.manager.free_request("a")
+    eng.runner.raise_on_device_error()
