@@ -79,3 +79,13 @@ def test_bounded_waits_come_behind_the_wait_for_the_kernel_in_front():
         assert "mbar_wait" not in front and "mbar_try_wait" not in front, at.group(1)
         seen += "mbar_wait" in body
     assert seen == 2
+
+
+def test_instructions_of_pairs_of_ctas_are_wrapped_once():
+    """Loads, products and commits of cta_group::2 stand in the header that the kernels share, and nothing of that header is written again beside a kernel."""
+    shared = set(re.findall(r"__device__ __forceinline__ \w+ (\w+)\(", SOURCES["tcgen05.cuh"]))
+    assert {"tma_load_2d_pair", "umma_bf16_pair", "umma_commit_pair", "umma_bf16", "mbar_init"} <= shared
+    for name, text in SOURCES.items():
+        if name != "tcgen05.cuh":
+            assert not shared & set(re.findall(r"__device__ __forceinline__ \w+ (\w+)\(", text)), name
+            assert not re.search(r"(cp\.async\.bulk\.tensor\.2d|tcgen05\.mma|tcgen05\.commit)\.cta_group::2", text), name
