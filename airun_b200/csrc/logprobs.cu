@@ -78,7 +78,7 @@ __device__ __forceinline__ u64 mul_pair(u64 a, u64 b) {
 // What the chunk with the maximum adds up to is rounded to 2^-24 of its 1.  Where less than this is left of a whole row without the 1, the chunk is looked at
 // again (others_again).  Not so where logits are formed and used at once: to keep 32 of them until then costs 6 % of 2,048 rows x [151936, 512], and what is rounded
 // is the probability of the 31 ids beside the leading one, by less than the logits' own errors from a width of 512 on.
-#define FEW_OTHERS 0.0625f
+#define FEW_OTHERS 0.25f
 
 // N logits, of which none is larger than `most`; true where they have brought the maximum.  Two at a time: additions and products take half the issue slots that way.
 template <int N> __device__ __forceinline__ bool add_chunk(Run& r, const float (&x)[N], float most) {

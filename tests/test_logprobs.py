@@ -718,3 +718,68 @@ def test_refusals_of_sizes_beyond_32_bits_and_of_other_error_words(monkeypatch):
     for bad in (_Fake(1), _Fake(1, dtype=torch.int64), _Fake(2, dtype=torch.int32), _Fake(0, dtype=torch.int32)):
         with pytest.raises(ops.KernelError, match="one int32"):
             ops.token_logprobs(_Fake(4, 100), t, lp, err=bad)
+
+
+# ---------------------------------------------------------------- how exact the sums are
+def peaked_hidden(n, H, V, seed):
+    """Hidden rows whose logits have a spread of 1.3 and ten that stand out by 14 to 24 and less, as a trained model's do."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    w = (0.02 * torch.randn(V, H, generator=g, device=DEV))
+    h = torch.randn(n, H, generator=g, device=DEV)
+    ids = torch.randint(0, V, (n, 10), generator=g, device=DEV)
+    lead = 14 + 10 * torch.rand(n, 1, generator=g, device=DEV) - (0.8 + 0.8 * torch.rand(n, 10, generator=g, device=DEV)).cumsum(1)
+    rows = w[ids]
+    h += torch.einsum("nl,nlh->nh", lead / rows.square().sum(-1), rows)
+    return h.to(torch.bfloat16), w.to(torch.bfloat16), ids[:, 0].to(torch.int32)
+
+
+def entropy_error(n, H, V, calls):
+    """Root mean square over all rows of the entropies' relative errors against 64 bits."""
+    off = []
+    for seed in range(calls):
+        h, w, t = peaked_hidden(n, H, V, 1000 * n + seed)
+        got = head(h, w, t, 0)
+        lp = torch.log_softmax(h.double() @ w.double().t(), dim=1)
+        want = -(lp.exp() * lp).sum(1).cpu()
+        off.append((got[1].double() - want) / want)
+    return float(torch.cat(off).square().mean().sqrt())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,H,calls,limit", [(16, 4096, 4, 5.5e-7), (40, 4096, 4, 4e-6), (64, 4096, 4, 4e-6), (100, 4096, 4, 4e-6), (300, 4096, 2, 4e-6)])
+def test_head_sums_stay_in_parts(n, H, calls, limit):
+    """A logit near 20 is rounded to 2^-20 a step.  Up to 32 rows its parts of 64 and 128 values are added with compensation, so one such rounding is left, 3e-7 in the
+    mean square (measured 3.4e-7; 8.7e-7 without compensation).  More rows add their parts of 128 and 512 values plainly: up to 32 roundings of partial sums on the way to 20,
+    about 1e-6 (measured 0.9e-6 to 1.4e-6; one sum over all 4,096 values 1.1e-5).  An entropy of these rows is off by about what its leading logits are."""
+    assert entropy_error(n, H, 12000, calls) <= limit
+
+
+@pytest.mark.gpu
+def test_head_whole_sums_would_be_seen(monkeypatch):
+    """The measure above tells parts from one sum."""
+    from airun_b200.kernels import fast
+    plan = fast.plan_head
+    monkeypatch.setattr(fast, "plan_head", lambda *a, **k: plan(*a, **k)[:4] + (64,))
+    assert entropy_error(100, 4096, 12000, 2) > 4e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 24, 200])
+def test_tokens_beside_a_leading_one_are_summed_to_full_precision(n):
+    """One token has all but about 1e-3 of a row, 151,935 others the rest.  Their terms' d = x - m is about -17: d * log2(e) is off by 1.3e-8 of itself (the constant
+    as a float) and a rounding, which averages out, so terms by 2.3e-7; sums of terms of one sign, compensated and joined in a few steps, add about 1e-7.  Where a sum
+    holds the leading token's 1 too each step rounds by up to 6e-8 of it, 6e-5 of what is looked for."""
+    V, off = 151936, []
+    for seed in range(-(-24 // n)):
+        g = torch.Generator(device=DEV).manual_seed(7 * n + seed)
+        x = 1.3 * torch.randn(n, V, generator=g, device=DEV)
+        at = torch.randint(0, V, (n, 1), generator=g, device=DEV)
+        x.scatter_(1, at, torch.logsumexp(x, 1, keepdim=True) + 6 + 2 * torch.rand(n, 1, generator=g, device=DEV))
+        got = call(x, at[:, 0].to(torch.int32), 1)
+        d = x.double() - x.double().amax(1, keepdim=True)
+        rest = torch.where(d < 0, d.exp(), 0.0).sum(1)
+        lp = -torch.log1p(rest)
+        entropy = -lp - (d.exp() * d).sum(1) / (1 + rest)
+        off.append(torch.stack(((got[0].double() - lp.cpu()) / lp.cpu(), (got[1].double() - entropy.cpu()) / entropy.cpu(), (got[4][:, 0].double() - lp.cpu()) / lp.cpu())))
+    off = torch.cat(off, 1)
+    assert float(off.square().mean(1).sqrt().max()) <= 4e-7 and float(off.abs().max()) <= 1e-6, (off.square().mean(1).sqrt(), off.abs().max())
