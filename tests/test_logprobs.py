@@ -783,3 +783,27 @@ def test_tokens_beside_a_leading_one_are_summed_to_full_precision(n):
         off.append(torch.stack(((got[0].double() - lp.cpu()) / lp.cpu(), (got[1].double() - entropy.cpu()) / entropy.cpu(), (got[4][:, 0].double() - lp.cpu()) / lp.cpu())))
     off = torch.cat(off, 1)
     assert float(off.square().mean(1).sqrt().max()) <= 4e-7 and float(off.abs().max()) <= 1e-6, (off.square().mean(1).sqrt(), off.abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [16, 40, 100, 300])
+def test_head_beside_a_leading_one(n):
+    """The same from hidden states with exact logits: multiples of 1/8 from -14 to -18 under a leading 0, 20,000 ids.  A term: d * log2(e) is 20 to 26 and rounded by 2^-20
+    at most, 6.6e-7 of the exponential, the constant is off by 1.3e-8 of itself, 2.4e-7 at 18, the exponential by 2^-22: 1.2e-6, the same for all ids of a logit, and
+    2e-7 for the sums.  More than 32 rows also add the 31 ids beside the leading one to its 1, in two chains of 16 additions that each round by 2^-24 at most."""
+    V, g = 20000, torch.Generator().manual_seed(n)
+    w = torch.zeros(V, 64)
+    w[:, :32] = -14 - torch.randint(0, 33, (V, 32), generator=g) / 8
+    at = torch.randint(0, V, (32,), generator=g)
+    w[at, torch.arange(32)] = 0.0
+    col = torch.arange(n) % 32
+    h = torch.zeros(n, 64)
+    h[torch.arange(n), col] = 1.0
+    got = head(h.to(torch.bfloat16).to(DEV), w.to(torch.bfloat16).to(DEV), at[col].to(torch.int32).to(DEV), 1)
+    x = w.double().t()[col]
+    rest = torch.where(x < 0, x.exp(), 0.0).sum(1)
+    lp = -torch.log1p(rest)
+    entropy = -lp - (x.exp() * x).sum(1) / (1 + rest)
+    for found, want in ((got[0], lp), (got[1], entropy), (got[2], -lp), (got[4][:, 0], lp)):
+        fine = ((found.double() - want).abs() <= 1.4e-6 * want.abs() + (2.0 ** -20 if n > 32 else 0.0)).all()
+        assert bool(fine), float(((found.double() - want).abs() / want.abs()).max())
