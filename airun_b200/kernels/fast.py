@@ -391,9 +391,9 @@ HEAD_TOP = 16                          # most alternatives that the fused head k
 def plan_head(n: int, V: int, K: int, sms: int = B200_SMS) -> Tuple[bool, int, int, int, int]:
     """(pairs of SMs, ranges of the vocabulary, tiles of a range, ids of a tile, K-steps of a part of a sum) for the log probabilities of n rows.
 
-    Up to 128 rows an SM to all of them, as the weights' bytes are the bound; up to 64 sums in parts of 128 values cost nothing (few rows
-    x 4,096 184 us for 187 in parts of 512, entropies off by 0.8e-6 for 2.2e-6), 100 rows with five alternatives take 140 us for 133.  Above, by the clocks of
-    the rounds that blocks of 128 rows (256 for a pair) and ranges take: 3 an id and K-step, 4 % less on pairs, whose tiles cost 2,500 more
+    Up to 128 rows an SM to all of them, as the weights' bytes are the bound.  Up to 64 sums in parts of 128 values: entropies off by 0.7e-6 for 2.4e-6 in parts of
+    512, for 1 % without alternatives (33 rows x 4,096 200 us for 199, 64 rows 203 for 201) and 8 to 14 % with five (64 rows x 4,096 226 for 209, x 2,048 136 for
+    120); 100 rows with five 143 for 125.  Above, by the clocks of the rounds that blocks of 128 rows (256 for a pair) and ranges take: 3 an id and K-step, 4 % less on pairs, whose tiles cost 2,500 more
     where K is too short to hide them; 6,000 a range, and 5 % a round for SMs that no longer read the same weights at the same time (2,048 x 4,096 on pairs in
     9, 18 and 46 ranges, one, two and five rounds: 1,596, 1,652 and 1,709).  B200, sustained, us, pairs and single SMs: 2,048 x 4,096 1,868 and 1,957; 4,095 x
     2,048 1,888 and 1,950; 2,048 x 512 309 and 240; with fewer rows that are not there, 300 x 4,096 479 and 376, 640 x 2,048 386 and 294 (151,936 ids all)."""
@@ -423,10 +423,12 @@ def plan_head(n: int, V: int, K: int, sms: int = B200_SMS) -> Tuple[bool, int, i
 HEAD_FEW = 32                          # most rows whose logits are written (both forms' times stand at head_few_kernel)
 
 
-def plan_few(V: int, sms: int = B200_SMS) -> Tuple[int, int]:
-    """(tiles of a range, ids of a tile): a range of the vocabulary an SM, in even tiles of up to 128 ids."""
+def plan_few(V: int, sms: int = B200_SMS, rows: int = 1) -> Tuple[int, int]:
+    """(tiles of a range, ids of a tile): a range of the vocabulary an SM, in even tiles of up to 128 ids, and no more than leave room for three stages with the rows'
+    (with two, 25 to 32 rows x [151936, 4096] 225 us)."""
     per = (V + sms - 1) // sms
-    tiles = (per + 127) // 128
+    most = min(128, 144 - (rows + 7) // 8 * 8)
+    tiles = (per + most - 1) // most
     return tiles, max(8, (per + tiles - 1) // tiles)
 
 
@@ -441,7 +443,7 @@ def head_logprobs_bf16(hidden, weight, tokens, logprob, entropy, lse, top_ids, t
         return False
     at, ldx, ldw = ops._at, hidden.stride(0) if n > 1 else max(K, hidden.stride(0)), weight.stride(0) if V > 1 else max(K, weight.stride(0))
     if n <= HEAD_FEW:
-        tiles, bn = plan_few(V, machine(hidden.device).sms)
+        tiles, bn = plan_few(V, machine(hidden.device).sms, n)
         ld = (V + 3) // 4 * 4
         logits = alloc((4 * n * ld,), torch.uint8)
         f = _fn("logprobs", "airun_head_few", _HEAD_FEW)

@@ -807,3 +807,16 @@ def test_head_beside_a_leading_one(n):
     for found, want in ((got[0], lp), (got[1], entropy), (got[2], -lp), (got[4][:, 0], lp)):
         fine = ((found.double() - want).abs() <= 1.4e-6 * want.abs() + (2.0 ** -20 if n > 32 else 0.0)).all()
         assert bool(fine), float(((found.double() - want).abs() / want.abs()).max())
+
+
+def test_plan_of_few_rows_leaves_room_for_three_stages():
+    """A stage of head_few_kernel holds four K-steps of 64 values of a tile's ids and of the rows, in groups of eight; the products read 128 ids and 16 or 32 rows from
+    the last ones on.  227 KB, of which one aligns the stages."""
+    from airun_b200.kernels.fast import HEAD_FEW, plan_few
+    up = lambda x: -(-x // 8) * 8      # noqa: E731
+    for rows in range(1, HEAD_FEW + 1):
+        for V in (1, 300, 2049, 20000, 32000, 50001, 128256, 151936, 262144):
+            tiles, bn = plan_few(V, 148, rows)
+            assert 1 <= bn <= 128 and -(-V // (tiles * bn)) <= 148
+            beyond = 128 * ((16 if rows <= 16 else 32) - up(rows) + 128 - up(bn))
+            assert 3 * 4 * 128 * (up(bn) + up(rows)) + beyond <= 230400 - 1024, (rows, V)
