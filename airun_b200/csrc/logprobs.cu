@@ -20,8 +20,7 @@ typedef unsigned long long u64;
 #define LOWEST (-200.0f)               // exp is 0 from here on, and so is a term's part in u
 
 // A part's s without the 1 that its maximum stands for: where one token leads, s is 1 and a little, and each addition would round the little, and with it the
-// entropy, to 2^-24 of the 1.  Entropies of 300 single rows of 151,936: relative errors up to 5e-7, 0.9e-7 in the mean square; 10e-7 and 1.5e-7 with s itself;
-// joined in 64 bits 5e-7 and 0.9e-7, but 7.2 us a row for 6.9.
+// entropy, to 2^-24 of the 1.  Entropies of single rows of 151,936 were off by 1.5e-7 in the mean square with s itself, 0.8e-7 now.
 struct Part { float m, rest, u; };
 
 __device__ __forceinline__ float exp_of(float d) {
@@ -642,9 +641,9 @@ template <int N> struct TopList {
 };
 template <> struct TopList<0> {};
 
-// cap * tanh(x / cap).  tanh z = 1 - 2 / (e^2z + 1), off by 2^-24 or so; below 1/4, where that would be many units, the odd series to z^9
-// (the next term is below 3e-9).  Without branches: 700 rows x [20000, 1024] take 43 us with it, 134 with
-// tanhf, which has some, and a division.
+// cap * tanh(x / cap).  tanh z = 1 - 2 / (e^2z + 1), where the exponential is off by 2^-22 of itself and the reciprocal by 2^-23: 2^-21 of the cap at most, 4.3 times
+// 2^-24 in 2.6 million logits; below 1/4, where that would be many units, the odd series to z^9 (the next term is below 3e-9).  A logit near 7 under a cap of 30 is off by
+// 6e-7 so, by what its product is off by too.  700 rows x [20000, 1024] take 37 us with it, 39 with tanhf; 2,048 x [20000, 512] 59 and 65.
 __device__ __forceinline__ float capped(float x, float cap, float over_cap) {
     const float z = x * over_cap, q = z * z;
     const float near = fmaf(z * q, fmaf(q, fmaf(q, fmaf(q, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), z);
@@ -655,8 +654,8 @@ __device__ __forceinline__ float capped(float x, float cap, float over_cap) {
 }
 
 // ROLLED: the epilogue's code, which runs once a tile and comes cold, is a quarter as long.  Unrolled it saves the moves, which only pays where tiles follow each
-// other fast: us, rolled and not, 2,048 rows x [151936, 2048] 992, 971; 5 rows x [151936, 4096] with five alternatives 211, 219; 700 rows x [20000, 1024]
-// capped 39, 44.
+// other fast: us, rolled and not, 2,048 rows x [151936, 2048] 950, 924, with five alternatives 996, 979; 64 rows x [151936, 4096] with five 215, 224; 100 rows x
+// [151936, 2048] with five 117, 125; capped, 700 rows x [20000, 1024] 37, 40, with five 57, 67.
 template <bool PAIR, int TOP, bool ROLLED>
 __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
     const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const HeadParams p) {
