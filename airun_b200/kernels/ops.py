@@ -1328,13 +1328,15 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Te
         raise KernelError(f"logits of at most {LOGITS_MAX} rows and columns, for at most {LOGPROB_ROWS_MAX} tokens")
     k = _logprob_outputs(n, V, tokens, logprob, entropy, lse, top_ids, top_logprobs)
     if rows is None:
-        _need(R >= n, "a row of logits for every token")
-    else:
-        _need(rows.dtype == torch.int32 and rows.shape == (n,) and rows.is_contiguous() and (R > 0 or n == 0), "rows must be int32 [n], of one row of logits or more")
-    if err is not None:
-        _need(err.dtype == torch.int32 and err.numel() == 1, "err must be one int32")
+        if R < n:
+            raise KernelError("a row of logits for every token")
+    elif rows.dtype != torch.int32 or rows.shape != (n,) or not rows.is_contiguous() or R == 0 and n > 0:
+        raise KernelError("rows must be int32 [n], of one row of logits or more")
+    if err is not None and (err.dtype != torch.int32 or err.numel() != 1):
+        raise KernelError("err must be one int32")
     ld = logits.stride(0) if R > 1 else V
-    _need(ld >= V, "rows of logits must not overlap")
+    if ld < V:
+        raise KernelError("rows of logits must not overlap")
     f = _fn("logprobs", "airun_token_logprobs", _TOKEN_LOGPROBS)
     _check(f(logits.data_ptr(), _dt(logits), ld, R, V, _at(rows), tokens.data_ptr(), n, logprob.data_ptr(), _at(entropy), _at(lse), k, _at(top_ids),
              _at(top_logprobs), _at(err), _stream(device)), "token_logprobs")
