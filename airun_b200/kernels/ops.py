@@ -1367,7 +1367,8 @@ def head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tens
     _dt(hidden)
     _need(hidden.stride(1) == 1 and weight.stride(1) == 1, "hidden and weight must be row-major")
     n, V = hs[0], wsh[0]
-    _need(max(V, hs[1]) <= LOGITS_MAX and n <= LOGPROB_ROWS_MAX, f"at most {LOGPROB_ROWS_MAX} rows, and {LOGITS_MAX} tokens and values")
+    if V > LOGITS_MAX or hs[1] > LOGITS_MAX or n > LOGPROB_ROWS_MAX:
+        raise KernelError(f"at most {LOGPROB_ROWS_MAX} rows, and {LOGITS_MAX} tokens and values")
     _need((n <= 1 or hidden.stride(0) >= hs[1]) and (V <= 1 or weight.stride(0) >= hs[1]), "rows of hidden and weight must not overlap")
     _need(tokens.dim() == 1 and tokens.shape[0] == n, "a token for every row")
     _logprob_outputs(n, V, tokens, logprob, entropy, lse, top_ids, top_logprobs)

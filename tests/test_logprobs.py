@@ -820,3 +820,29 @@ def test_plan_of_few_rows_leaves_room_for_three_stages():
             assert 1 <= bn <= 128 and -(-V // (tiles * bn)) <= 148
             beyond = 128 * ((16 if rows <= 16 else 32) - up(rows) + 128 - up(bn))
             assert 3 * 4 * 128 * (up(bn) + up(rows)) + beyond <= 230400 - 1024, (rows, V)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,n", [(301, 1), (2047, 3), (20003, 1), (20003, 5), (20003, 150), (70001, 1)])
+def test_tokens_peaked_rows_that_start_and_end_between_vectors(V, n, dtype):
+    """Leading and second tokens among the elements ahead of the first 16-byte boundary and behind the last one, which belong to the first and the last block; rows are
+    picked, every one at another distance from a boundary, with large logits beside them."""
+    places = [0, 1, 2, 6, 8, V - 9, V - 5, V - 2, V - 1]
+    pairs = [(a, b, d) for a in places for b in places if a != b for d in APART[:1 + 2 * (n == 1)]]
+    buf = torch.full((len(pairs), V + 5), 50.0)
+    x = buf[:, 3:3 + V]
+    x[:] = -math.inf
+    for r, (a, b, d) in enumerate(pairs):
+        x[r, a], x[r, b] = 0.0, -d
+    x = buf.to(dtype).to(DEV)[:, 3:3 + V]
+    g = torch.Generator().manual_seed(V)
+    order = torch.randperm(len(pairs), generator=g).tolist()
+    order = (order * (1 + n // len(order)))[:max(len(order) // n * n, n)]
+    for at in range(0, len(order), n):
+        rows = order[at:at + n]
+        leads = torch.tensor([(at + i) % 2 == 0 for i in range(n)])
+        t = torch.tensor([pairs[r][0 if leads[i] else 1] for i, r in enumerate(rows)], dtype=torch.int32, device=DEV)
+        got = call(x, t, 2, torch.tensor(rows, dtype=torch.int32, device=DEV))
+        check_peaked(got, [pairs[r][2] for r in rows], leads)
+        assert got[3].tolist() == [[pairs[r][0], pairs[r][1]] for r in rows]
