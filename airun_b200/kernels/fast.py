@@ -423,6 +423,7 @@ def plan_head(n: int, V: int, K: int, sms: int = B200_SMS) -> Tuple[bool, int, i
 HEAD_FEW = 32                          # most rows whose logits are written (both forms' times stand at head_few_kernel)
 
 
+@lru_cache(maxsize=4096)
 def plan_few(V: int, sms: int = B200_SMS, rows: int = 1) -> Tuple[int, int]:
     """(tiles of a range, ids of a tile): a range of the vocabulary an SM, in even tiles of up to 128 ids, and no more than leave room for three stages with the rows'
     (with two, 25 to 32 rows x [151936, 4096] 225 us)."""
