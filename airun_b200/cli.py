@@ -265,7 +265,7 @@ def cmd_bench(a) -> int:
     return 0
 
 
-LOSS_BLOCK = 1 << 25                   # logits that are held in 64 bits at a time: 256 MiB
+LOSS_BLOCK = 1 << 26                   # logits that are taken to 64 bits at a time: 512 MiB, and as much for their log probabilities
 
 
 def place_losses(logits, targets):
@@ -280,9 +280,9 @@ def place_losses(logits, targets):
     for at in range(0, n, step):
         t = want[at:at + step]
         rows = logits[at:at + step]
-        losses += (-torch.log_softmax(rows.double(), dim=-1).gather(1, t[:, None])[:, 0]).tolist()
-        best += (rows.argmax(dim=-1) == t).tolist()
-    return losses, best
+        losses.append(-torch.log_softmax(rows.double(), dim=-1).gather(1, t[:, None])[:, 0])
+        best.append(rows.argmax(dim=-1) == t)
+    return torch.cat(losses).tolist(), torch.cat(best).tolist()
 
 
 def cmd_perplexity(a) -> int:
