@@ -659,7 +659,6 @@ __device__ __forceinline__ float capped(float x, float cap, float over_cap) {
 template <bool PAIR, int TOP, bool ROLLED>
 __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
     const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const HeadParams p) {
-    pdl_trigger();
     constexpr int CTAS = PAIR ? 2 : 1;
     __shared__ __align__(8) uint64_t bars[2 * HEAD_STAGES + 4];    // full (a pair: the leader's), empty of the stages; full, empty (the leader's) of the sums
     __shared__ uint32_t tmem_slot;
@@ -689,6 +688,7 @@ __global__ __launch_bounds__(HEAD_THREADS, 1) void head_logprobs_kernel(
     tc_fence_before();
     __syncthreads();
     if constexpr (PAIR) cluster_sync_all();                        // the leader's barriers are there before anything arrives at them
+    pdl_trigger();                                                 // (not sooner: a kernel behind could take the tensor memory and wait for this one)
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     const uint32_t full_lead = PAIR ? map_to_cta(full, 0) : full, acce_lead = PAIR ? map_to_cta(acce, 0) : acce;
@@ -1095,7 +1095,6 @@ struct FewParams {
 
 template <int N>
 __global__ __launch_bounds__(FEW_THREADS, 1) void head_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const FewParams p) {
-    pdl_trigger();
     __shared__ __align__(8) uint64_t bars[2 * FEW_STAGES + 2 * FEW_BUFS];
     __shared__ uint32_t tmem_slot;
     extern __shared__ uint8_t smem_raw[];
@@ -1116,6 +1115,7 @@ __global__ __launch_bounds__(FEW_THREADS, 1) void head_few_kernel(const __grid_c
     if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), FEW_BUFS * COLS);
     tc_fence_before();
     __syncthreads();
+    pdl_trigger();                                                 // (as above)
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     const int n_steps = (end_id - first_id + p.bn - 1) / p.bn * kb_total, first_n = min(n_steps, stages);
@@ -1238,7 +1238,9 @@ static int launch_few(const CUtensorMap& mx, const CUtensorMap& mw, FewParams p,
     const int beyond_x = N * BK * 2 - p.x_bytes, beyond_w = 128 * BK * 2 - p.w_stride;
     p.stages = (HEAD_SMEM - 1024 - beyond_x - beyond_w) / (FEW_K * (p.w_stride + p.x_bytes));
     if (p.stages > FEW_STAGES) p.stages = FEW_STAGES;
-    const int smem = 1024 + p.stages * FEW_K * (p.w_stride + p.x_bytes) + beyond_x + beyond_w;
+    // all of the SM's shared memory, whatever the stages need: a kernel in front that has not taken its own tensor memory yet must not meet this one on its SM, which would
+    // take it and wait for that kernel to end (head_logprobs_kernel has all of the SM's registers)
+    const int smem = HEAD_SMEM;
     if (first_on_device(configured)) {
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, HEAD_SMEM);
         if (e != cudaSuccess) { configured = 0; return (int)e; }

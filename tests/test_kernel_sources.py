@@ -89,3 +89,21 @@ def test_instructions_of_pairs_of_ctas_are_wrapped_once():
         if name != "tcgen05.cuh":
             assert not shared & set(re.findall(r"__device__ __forceinline__ \w+ (\w+)\(", text)), name
             assert not re.search(r"(cp\.async\.bulk\.tensor\.2d|tcgen05\.mma|tcgen05\.commit)\.cta_group::2", text), name
+
+
+def test_heads_hold_their_tensor_memory_before_others_may_start():
+    """A kernel behind may be resident as soon as every block has passed pdl_trigger().  If it could take tensor memory that a block in front still has to ask for, it would
+    wait for that block to end, and the block for the memory.  So the heads take theirs first, and the one that leaves registers free leaves no shared memory
+    beside a kernel in front."""
+    text, seen = SOURCES["logprobs.cu"], 0
+    for at in re.finditer(r"__global__[^;{]*?\bvoid\s+(\w+)\s*\(", text):
+        body = text[at.end():text.find("\n}\n", at.end())]
+        if "tmem_alloc(" in body:
+            seen += 1
+            assert body.rindex("tmem_alloc(") < body.index("__syncthreads()") < body.index("pdl_trigger()") < body.index("pdl_wait()"), at.group(1)
+    assert seen == 2
+    few = text[text.index("static int launch_few("):]
+    assert "const int smem = HEAD_SMEM;" in few[:few.index("\n}\n")]
+    from math import ceil
+    regs = int(re.search(r"#define HEAD_REGS (\d+)", text).group(1)) * int(re.search(r"#define HEAD_THREADS (\d+)", text).group(1))
+    assert 65536 - regs < 32 * 40 and ceil(regs / 65536) == 1      # (no second block of a warp with 40 registers)
