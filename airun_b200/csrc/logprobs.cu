@@ -1072,8 +1072,8 @@ AIRUN_EXPORT int airun_head_logprobs(const void* x, const void* W, int n, int V,
 // token_logprobs_kernel takes them from the L2.  A block walks a range of the vocabulary in tiles of `bn` <= 128 ids, of any number, so that the ranges come
 // out even.  us, this and head_logprobs_kernel, weights of [151936, 4096] on a cool chip: 5 rows 191 and 190, with five alternatives 198 and 203; 24 rows 201 and 194, with eight
 // 207 and 213; 32 rows 206 and 204, with eight 213 and 211; on a hot one 5 rows 202 and 196, with five 211 and 232, 32 rows 223 and 218, with eight 223 and 233.  5 rows x
-// [20000, 1024] 13.0 and 14.6, 32 rows with five 18.9 and 28.4; 32 rows x [384, 64] 6.4 and 5.2, with three 8.8 and 10.2.  Up to 3.5 % slower without
-// alternatives, up to a third faster with them, and its sums are the more exact.
+// [20000, 1024] 13.0 and 14.6, 32 rows with five 18.9 and 28.4; 32 rows x [384, 64] 6.4 and 5.2, with three 8.8 and 10.2.  Without alternatives up to
+// 3.5 % slower where weights are many, with them up to a third faster, and its sums are the more exact.
 //   warp 0: TMA loads; warp 1: tensor memory, products; warps 2-5: the sums of a quadrant of lanes each, one id a thread.
 // A stage is FEW_K K-steps, and its sums are parts of 64 values (128 for more than 16 rows) in neighbouring columns that are loaded together: a load takes 1,100
 // clocks whatever its width.  (Stages of one K-step 237 us for 5 rows, of two 197.)  The stages' sums are added with compensation: entropies of 5 rows x 4,096
