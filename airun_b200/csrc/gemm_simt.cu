@@ -480,6 +480,8 @@ __global__ __launch_bounds__(X_THREADS, 1) void gemm_f32_parts_kernel(
 
     const int cols = min(bn, m_end - m0);
     float* sums = reinterpret_cast<float*>(tiles);             // of this slice, [column][128], once the products are done
+    const bool loads = warp == X_SUM_WARPS + X_CUT_WARPS + 1;
+    if (FORM != 2 && !loads) pdl_wait();                       // the waits below are bounded, the kernel in front is not; the loads of weights come ahead of it
     if (warp < X_SUM_WARPS) {
         const int quad = warp & 3, half = warp >> 2;
         float2 acc[XB / 4];                                    // columns 16 (2 j + half) + 2 i and the next at [8 j + i]

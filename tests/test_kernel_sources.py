@@ -68,17 +68,27 @@ def test_kernels_wait_before_they_end_and_trigger_first():
 
 def test_bounded_waits_come_behind_the_wait_for_the_kernel_in_front():
     """A wait on a barrier gives up after two seconds, but the kernel in front may run for longer: a warp that stood at a barrier meanwhile, for operands that another
-    warp asks for behind its pdl_wait(), would report a wait that has run out.  In the kernels of log probabilities every warp passes pdl_wait() first, once and for
-    all roles."""
-    text, seen = SOURCES["logprobs.cu"], 0
-    for at in re.finditer(r"__global__[^;{]*?\bvoid\s+(\w+)\s*\(", text):
-        end = text.find("\n}\n", at.end())
-        body = text[at.end():end]
-        assert body.count("pdl_wait();") == 1 and re.search(r"^    pdl_wait\(\);", body, re.M), at.group(1)
-        front = body[:body.index("pdl_wait();")]
-        assert "mbar_wait" not in front and "mbar_try_wait" not in front, at.group(1)
-        seen += "mbar_wait" in body
-    assert seen == 2
+    warp asks for behind its pdl_wait(), would report a wait that has run out.  Every warp passes pdl_wait() first, most once and for all roles."""
+    seen = set()
+    for name, text in SOURCES.items():
+        for at in re.finditer(r"__global__[^;{]*?\bvoid\s+(\w+)\s*\(", text):
+            body = text[at.end():text.find("\n}\n", at.end())]
+            if not re.search(r"\bmbar_(try_)?wait", body):
+                continue
+            seen.add(at.group(1))
+            if at.group(1) == "attn_decode_kernel":                # one flow for all threads, which waits early or behind the first loads
+                front = body[:body.rindex("pdl_wait();")]
+            elif at.group(1) == "gemm_f32_parts_kernel":           # the last role, the loads', asks for weights first
+                assert "const bool loads = warp == X_SUM_WARPS + X_CUT_WARPS + 1;" in body and "if (FORM != 2 && !loads) pdl_wait();" in body
+                front = body[:body.index("!loads) pdl_wait();")]
+                role = body[body.index("auto ask = "):]
+                assert "mbar_wait" not in role[:role.index("if (FORM != 2) pdl_wait();")]
+            else:
+                wait = re.search(r"^    pdl_wait\(\);", body, re.M)
+                assert wait and body.count("pdl_wait();") == 1, at.group(1)
+                front = body[:wait.start()]
+            assert not re.search(r"\bmbar_(try_)?wait", front), at.group(1)
+    assert {"head_logprobs_kernel", "head_few_kernel", "gemm_f32_parts_kernel", "gemm_pair_kernel", "attn_decode_kernel", "latent_prefill_kernel"} <= seen
 
 
 def test_instructions_of_pairs_of_ctas_are_wrapped_once():
@@ -104,6 +114,5 @@ def test_heads_hold_their_tensor_memory_before_others_may_start():
     assert seen == 2
     few = text[text.index("static int launch_few("):]
     assert "const int smem = HEAD_SMEM;" in few[:few.index("\n}\n")]
-    from math import ceil
     regs = int(re.search(r"#define HEAD_REGS (\d+)", text).group(1)) * int(re.search(r"#define HEAD_THREADS (\d+)", text).group(1))
-    assert 65536 - regs < 32 * 40 and ceil(regs / 65536) == 1      # (no second block of a warp with 40 registers)
+    assert 0 <= 65536 - regs < 32 * 40                             # (no second block of a warp with 40 registers)
