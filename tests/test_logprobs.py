@@ -846,3 +846,22 @@ def test_tokens_peaked_rows_that_start_and_end_between_vectors(V, n, dtype):
         got = call(x, t, 2, torch.tensor(rows, dtype=torch.int32, device=DEV))
         check_peaked(got, [pairs[r][2] for r in rows], leads)
         assert got[3].tolist() == [[pairs[r][0], pairs[r][1]] for r in rows]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [32, 20000])
+@pytest.mark.parametrize("cap", [5.0, 30.0])
+def test_capped_logits_by_themselves(n, cap):
+    """A vocabulary of one id: ln sum exp is the capped logit, with no rounding beside it.  From 1/4 of a cap on: the exponential's argument is 2 z log2(e) with
+    z, the constant and the product rounded (4 times 2^-24 of it), tanh falls by z sech^2 z <= 0.45 of that; the exponential (2^-22 of itself, times at most 0.47 = 2 e / (e + 1)^2), the
+    reciprocal (2^-23, times 0.76) and two roundings come to 1.8 times 2^-22 of the cap with it; below 1/4 three or four roundings of the series, of up to 1/4 of the cap."""
+    w = torch.zeros(1, 8, device=DEV, dtype=torch.bfloat16)
+    w[0, 0] = 1.0
+    g = torch.Generator(device=DEV).manual_seed(n)
+    for scale in (1.0, 1.01171875, 0.1):
+        h = torch.zeros(n, 8, device=DEV, dtype=torch.bfloat16)
+        h[:, 0] = ((torch.rand(n, generator=g, device=DEV) * 2 - 1) * 4 * cap).to(torch.bfloat16)
+        got = head(h, w, torch.zeros(n, dtype=torch.int32, device=DEV), 0, scale, cap)
+        z = (h[:, 0].float() * torch.tensor(scale, device=DEV)).double().cpu() / cap
+        assert float((got[2].double() - cap * torch.tanh(z)).abs().max()) <= cap * 1.8 * 2.0 ** -22
+        assert bool((got[0] == 0).all()) and bool((got[1] == 0).all())
