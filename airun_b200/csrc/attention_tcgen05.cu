@@ -225,7 +225,6 @@ template <bool SHARED, bool SPLIT>
 __global__ __launch_bounds__(TC_THREADS, 1) void attn_prefill_tc_kernel(
     const TcParams p, const int4* tiles, const __grid_constant__ CUtensorMap kv_map,
     const int* n_tiles_dev, const TcShared sh) {
-    pdl_trigger();
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* bars = (uint64_t*)(smem + OFF_BAR);
@@ -248,6 +247,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void attn_prefill_tc_kernel(
     if (warp == 1) tmem_alloc(smem_u32(tmem_slot), 512);
     tc_fence_before();
     __syncthreads();
+    pdl_trigger();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     auto leave = [&]() {
@@ -717,7 +717,6 @@ __global__ __launch_bounds__(TC_THREADS, 1) void attn_prefill_wide_kernel(
     // what a hidden key's score is and the lowest a row's maximum counts from: with a distance table a visible score may be as
     // low as float32 goes
     constexpr float HIDDEN = KIND == W_PLAIN ? NEG_BIG : -INFINITY, LOWEST = KIND == W_PLAIN ? 0.5f * NEG_BIG : -INFINITY;
-    pdl_trigger();
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* bars = (uint64_t*)(smem + W_OFF_BAR);
@@ -738,6 +737,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void attn_prefill_wide_kernel(
     if (warp == 1) tmem_alloc(smem_u32(tmem_slot), 512);
     tc_fence_before();
     __syncthreads();
+    pdl_trigger();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     pdl_wait();

@@ -29,7 +29,9 @@
 // the kernel before it in the stream is still running; it must call pdl_wait() before it touches
 // global memory that an earlier kernel writes or reads (the wait returns when the earlier kernels
 // have finished and their writes are visible).  Every kernel calls pdl_trigger() first, which lets
-// the kernel after it become resident as soon as room is free.  What a kernel does before
+// the kernel after it become resident as soon as room is free; one that needs tensor memory calls it
+// once it has that: the kernel after it could otherwise take the tensor memory of an SM where a block
+// of this one is still to ask, and each would wait for the other.  What a kernel does before
 // pdl_wait() (shared-memory barriers, tensor-memory allocation, loads of WEIGHTS and of the batch's
 // layout, which no kernel of a step writes) overlaps the tail of the kernel before it.  AIRUN_PDL=0 in
 // the environment turns it off.

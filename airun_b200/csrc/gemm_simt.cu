@@ -439,7 +439,7 @@ template <int FORM>                                            // 0 plain, 2 gro
 __global__ __launch_bounds__(X_THREADS, 1) void gemm_f32_parts_kernel(
     const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float* A, const float* __restrict__ W,
     float* __restrict__ C, int M, int N, int K, long long lda, long long ldw, long long ldc, GemmExtra ex, int bn, int ks, int* err) {
-    pdl_trigger();
+    pdl_trigger();                                             // (ahead of its tensor memory: with X_SMEM no other kernel that asks for some fits beside it)
     extern __shared__ uint8_t x_raw[];
     uint8_t* tiles = (uint8_t*)(((uintptr_t)x_raw + 1023) & ~(uintptr_t)1023);
     // full, empty of the stages of parts; full, empty of the leading sum and of the other; landed, read of the ring

@@ -360,7 +360,6 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void gemm_tcgen05_kernel(
     // PUSH: the slices are brought together by stores (see push_slices)
     constexpr bool PUSH = CLUSTER && SWAP && !AIRUN_FOLD_NORM;
 
-    pdl_trigger();
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const int a0 = blockIdx.x * BM;            // first A row of the tile
     const int b0 = blockIdx.y * BN;            // first B row of the tile
@@ -383,6 +382,7 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void gemm_tcgen05_kernel(
     if (warp == 1) tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
     tc_fence_before();
     __syncthreads();
+    pdl_trigger();
     tc_fence_after();
     if (PUSH) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
@@ -714,7 +714,6 @@ template <int EPI, bool BATCHED>
 __global__ __launch_bounds__(P_THREADS, 1) void gemm_tcgen05_persistent_kernel(
     const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmParams p,
     int m_tiles, int n_tiles) {
-    pdl_trigger();
     using L = SmemLayout<PBN, PSTAGES>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -734,6 +733,7 @@ __global__ __launch_bounds__(P_THREADS, 1) void gemm_tcgen05_persistent_kernel(
     if (warp == 1) tmem_alloc(smem_u32(&tmem_slot_p), 2 * PBN);
     tc_fence_before();
     __syncthreads();
+    pdl_trigger();
     tc_fence_after();
     const uint32_t tmem_base = tmem_slot_p;
     // The weights (the B operand) are written by no kernel: the first stages of this CTA's first tile
@@ -952,7 +952,6 @@ __device__ __forceinline__ void store_pair(const GemmParams& p, const float* v, 
 template <int EPI, bool GROUPED, bool IN_PARTS>
 __global__ __launch_bounds__(PAIR_THREADS, 1) void gemm_pair_kernel(
     const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const GemmParams p, int bn, int tok_tiles) {
-    pdl_trigger();
     __shared__ int4 s_tab[GROUPED ? GROUP_MAX_TILES : 1];          // first row, end of the segment, segment, width
     __shared__ int s_first[GROUPED ? GROUP_MAX_SEGS + 1 : 1];
     __shared__ __align__(8) uint64_t bars[2 * PAIR_STAGES + 4];    // full (the leader's), empty of the stages; full, empty (the leader's) of the sums
@@ -975,6 +974,7 @@ __global__ __launch_bounds__(PAIR_THREADS, 1) void gemm_pair_kernel(
     }
     tc_fence_before();
     __syncthreads();
+    pdl_trigger();
     cluster_sync_all();                                            // the leader's barriers are there before anything arrives at them
     tc_fence_after();
     const uint32_t tmem = tmem_slot;

@@ -94,7 +94,6 @@ enum { L_QFULL = 0, L_NFULL = 1, L_NEMPTY = 3, L_VFULL = 5, L_VEMPTY = 7, L_SFUL
 __global__ __launch_bounds__(LT_THREADS, 1) void latent_prefill_kernel(
     const LatParams p, const int4* tiles, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
     const int* n_tiles_dev) {
-    pdl_trigger();
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* const smem_k = smem + p.blocks * LT_QBLK;
@@ -111,6 +110,7 @@ __global__ __launch_bounds__(LT_THREADS, 1) void latent_prefill_kernel(
     if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), 512);
     tc_fence_before();
     __syncthreads();
+    pdl_trigger();
     tc_fence_after();
     const uint32_t tmem_base = tmem_slot;
     const uint32_t tmem_o = tmem_base + 2 * LT_KEYS;

@@ -101,18 +101,21 @@ def test_instructions_of_pairs_of_ctas_are_wrapped_once():
             assert not re.search(r"(cp\.async\.bulk\.tensor\.2d|tcgen05\.mma|tcgen05\.commit)\.cta_group::2", text), name
 
 
-def test_heads_hold_their_tensor_memory_before_others_may_start():
+def test_kernels_hold_their_tensor_memory_before_others_may_start():
     """A kernel behind may be resident as soon as every block has passed pdl_trigger().  If it could take tensor memory that a block in front still has to ask for, it would
-    wait for that block to end, and the block for the memory.  So the heads take theirs first, and the one that leaves registers free leaves no shared memory
-    beside a kernel in front."""
-    text, seen = SOURCES["logprobs.cu"], 0
-    for at in re.finditer(r"__global__[^;{]*?\bvoid\s+(\w+)\s*\(", text):
-        body = text[at.end():text.find("\n}\n", at.end())]
-        if "tmem_alloc(" in body:
-            seen += 1
-            assert body.rindex("tmem_alloc(") < body.index("__syncthreads()") < body.index("pdl_trigger()") < body.index("pdl_wait()"), at.group(1)
-    assert seen == 2
-    few = text[text.index("static int launch_few("):]
-    assert "const int smem = HEAD_SMEM;" in few[:few.index("\n}\n")]
-    regs = int(re.search(r"#define HEAD_REGS (\d+)", text).group(1)) * int(re.search(r"#define HEAD_THREADS (\d+)", text).group(1))
-    assert 0 <= 65536 - regs < 32 * 40                             # (no second block of a warp with 40 registers)
+    wait for that block to end, and the block for the memory.  So a kernel takes its own first."""
+    seen = set()
+    for name, text in SOURCES.items():
+        for at in re.finditer(r"__global__[^;{]*?\bvoid\s+(\w+)\s*\(", text):
+            body = text[at.end():text.find("\n}\n", at.end())]
+            asks = [m.start() for m in re.finditer(r"\btmem_alloc\(|tcgen05\.alloc\.", body)]
+            if asks:
+                seen.add(at.group(1))
+                trigger = body.index("pdl_trigger();")
+                if at.group(1) == "gemm_f32_parts_kernel":         # all but 4 KB of the shared memory is its own
+                    size = lambda n: int(eval(re.sub(r"[A-Z]\w+", lambda m: str(size(m.group(0))), re.search(rf"#define {n} ([^\n]*)", text).group(1))))      # noqa: E731
+                    assert 220 * 1024 <= size("X_SMEM") <= 227 * 1024
+                    continue
+                assert body.count("pdl_trigger();") == 1 and asks[-1] < trigger and "__syncthreads();" in body[asks[-1]:trigger], at.group(1)
+    assert {"head_logprobs_kernel", "head_few_kernel", "gemm_tcgen05_kernel", "gemm_tcgen05_persistent_kernel", "gemm_pair_kernel", "gemm_f32_parts_kernel",
+            "attn_prefill_tc_kernel", "attn_prefill_wide_kernel", "latent_prefill_kernel"} == seen
